@@ -95,6 +95,13 @@ class SynthConfig(ctypes.Structure):
                 ("anchors", ctypes.c_int32), ("seed", ctypes.c_uint64)]
 
 
+class KvPages(ctypes.Structure):
+    """gaje_hip_kv_pages; `buffers` (set by ops.kv_pages) keeps its memory alive."""
+    _fields_ = [("k", c_vp), ("v", c_vp), ("table", c_vp), ("len", c_vp), ("ref", c_vp), ("n_layer", c_i64),
+                ("n_pages", c_i64), ("n_seq", c_i64), ("max_pages", c_i64), ("dtype", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
 # (name, restype, argtypes): every symbol include/gaje_hip.h declares.
 SIGNATURES = [
     ("gaje_hip_last_error", ctypes.c_char_p, []),
@@ -147,6 +154,22 @@ SIGNATURES = [
     ("gaje_hip_expf", ctypes.c_int, [c_vp, c_vp, c_i64, c_vp]),
     ("gaje_hip_attention", ctypes.c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, ctypes.c_int, ctypes.c_int,
                                           ctypes.c_int, c_vp, c_vp]),
+    ("gaje_hip_kv_workspace", c_i64, [ctypes.POINTER(KvPages)]),
+    ("gaje_hip_kv_update", ctypes.c_int, [ctypes.POINTER(KvPages), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
+                                          c_vp]),
+    ("gaje_hip_kv_compact", ctypes.c_int, [ctypes.POINTER(KvPages), c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    ("gaje_hip_kv_append", ctypes.c_int, [ctypes.POINTER(KvPages), c_i64, ctypes.c_int, c_vp, c_i64, c_vp, c_i64,
+                                          c_vp, c_i64, c_vp]),
+    ("gaje_hip_attention_packed_workspace", c_i64, [c_i64, c_i64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    ("gaje_hip_attention_packed", ctypes.c_int, [ctypes.c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
+                                                 c_i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
+                                                 c_vp, c_i64, c_vp, c_i64, c_vp]),
+    ("gaje_hip_attention_paged_workspace", c_i64, [ctypes.POINTER(KvPages), c_i64, ctypes.c_int]),
+    ("gaje_hip_attention_paged", ctypes.c_int, [c_vp, c_i64, ctypes.POINTER(KvPages), c_i64, c_vp, c_i64,
+                                                ctypes.c_int, ctypes.c_float, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    ("gaje_hip_attention_prefix_workspace", c_i64, [ctypes.POINTER(KvPages), c_i64, ctypes.c_int]),
+    ("gaje_hip_attention_prefix", ctypes.c_int, [c_vp, c_i64, ctypes.POINTER(KvPages), c_i64, c_vp, c_i64,
+                                                 ctypes.c_int, ctypes.c_float, c_vp, c_i64, c_vp, c_i64, c_vp]),
     ("gaje_hip_kwta", ctypes.c_int, [c_vp, c_i64, c_i64, c_vp]),
     ("gaje_hip_argmax", ctypes.c_int, [c_vp, c_i64, c_vp, c_vp]),
     ("gaje_hip_open", ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(c_vp)]),

@@ -7,7 +7,7 @@ import ctypes
 
 import numpy as np
 
-from ._lib import check, lib
+from ._lib import KvPages, check, lib
 
 
 class DeviceBuffer:
@@ -243,6 +243,86 @@ def attention(q: DeviceBuffer, k_cache: DeviceBuffer, v_cache: DeviceBuffer, seq
     """k_cache and v_cache are both [n_head_kv][head_dim][capacity]."""
     check(lib().gaje_hip_attention(q.ptr, k_cache.ptr, v_cache.ptr, seq_len, capacity, n_head,
                                    n_head_kv, head_dim, out.ptr, stream))
+
+
+# -- serving many sequences: a paged KV cache and the attention over it -------
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def kv_pages(k, v, table, length, ref, *, n_layer: int, n_pages: int, page: int, n_seq: int, max_pages: int,
+             n_head_kv: int, head_dim: int, dtype: str = "f32") -> KvPages:
+    """A paged KV cache over the caller's device buffers (gaje_hip_kv_pages): k and v
+    [n_layer][n_pages][page][n_head_kv][head_dim] of dtype, int32 table [n_seq][max_pages],
+    length [n_seq] and ref [n_pages].  ValueError if a buffer is too small."""
+    need = n_layer * n_pages * page * n_head_kv * head_dim * (4 if dtype == "f32" else 2)
+    for name, b, nbytes in (("k", k, need), ("v", v, need), ("table", table, 4 * n_seq * max_pages),
+                            ("length", length, 4 * n_seq), ("ref", ref, 4 * n_pages)):
+        if b.nbytes < nbytes:
+            raise ValueError(f"kv_pages: {name} has {b.nbytes} bytes, {nbytes} are needed")
+    c = KvPages(k.ptr, v.ptr, table.ptr, length.ptr, ref.ptr, n_layer, n_pages, n_seq, max_pages, DTYPES[dtype], page,
+                n_head_kv, head_dim)
+    c.buffers = (k, v, table, length, ref)
+    return c
+
+
+def kv_workspace(cache: KvPages) -> int:
+    return int(lib().gaje_hip_kv_workspace(cache))
+
+
+def kv_update(cache: KvPages, new_table, new_length, new_ref, status, workspace, source=None, add=None,
+              stream=None) -> None:
+    """Slots forked, freed, cut and grown: slot d becomes old slot source[d] (-1: empty), its
+    length changed by add[d]; the new arrays receive the result (gaje_hip_kv_update)."""
+    check(lib().gaje_hip_kv_update(cache, _p(source), _p(add), new_table.ptr, new_length.ptr, new_ref.ptr, status.ptr,
+                                   workspace.ptr, workspace.nbytes, stream))
+
+
+def kv_compact(cache: KvPages, new_table, new_ref, n_live, workspace, stream=None) -> None:
+    """The pages in use moved to the front of the pool (gaje_hip_kv_compact)."""
+    check(lib().gaje_hip_kv_compact(cache, new_table.ptr, new_ref.ptr, n_live.ptr, workspace.ptr, workspace.nbytes,
+                                    stream))
+
+
+def kv_append(cache: KvPages, layer: int, k, ldk: int, v, ldv: int, seq_off, T: int, source: str = "f32",
+              stream=None) -> None:
+    """One layer's new K and V rows into the cache's pages (gaje_hip_kv_append)."""
+    check(lib().gaje_hip_kv_append(cache, layer, DTYPES[source], k.ptr, ldk, v.ptr, ldv, seq_off.ptr, T, stream))
+
+
+def attention_packed_workspace(T: int, n_seq: int, n_head: int, n_head_kv: int, head_dim: int) -> int:
+    return int(lib().gaje_hip_attention_packed_workspace(T, n_seq, n_head, n_head_kv, head_dim))
+
+
+def attention_packed(q, ldq: int, k, ldk: int, v, ldv: int, seq_off, n_seq: int, T: int, n_head: int, n_head_kv: int,
+                     head_dim: int, scale: float, out, ldo: int, workspace, dtype: str = "f32", stream=None) -> None:
+    """Causal GQA attention of n_seq prompts packed row after row (gaje_hip_attention_packed)."""
+    check(lib().gaje_hip_attention_packed(DTYPES[dtype], q.ptr, ldq, k.ptr, ldk, v.ptr, ldv, seq_off.ptr, n_seq, T,
+                                          n_head, n_head_kv, head_dim, scale, out.ptr, ldo, workspace.ptr,
+                                          workspace.nbytes, stream))
+
+
+def attention_paged_workspace(cache: KvPages, T: int, n_head: int) -> int:
+    return int(lib().gaje_hip_attention_paged_workspace(cache, T, n_head))
+
+
+def attention_paged(q, ldq: int, cache: KvPages, layer: int, seq_off, T: int, n_head: int, scale: float, out, ldo: int,
+                    workspace, stream=None) -> None:
+    """Causal GQA attention of each sequence's last rows over its cached pages
+    (gaje_hip_attention_paged): single tokens, drafted tokens, a prompt's next chunk."""
+    check(lib().gaje_hip_attention_paged(q.ptr, ldq, cache, layer, seq_off.ptr, T, n_head, scale, out.ptr, ldo,
+                                         workspace.ptr, workspace.nbytes, stream))
+
+
+def attention_prefix_workspace(cache: KvPages, prefix_len: int, n_head: int) -> int:
+    return int(lib().gaje_hip_attention_prefix_workspace(cache, prefix_len, n_head))
+
+
+def attention_prefix(q, ldq: int, cache: KvPages, layer: int, prefix_table, prefix_len: int, n_head: int, scale: float,
+                     out, ldo: int, workspace, stream=None) -> None:
+    """One token of every sequence over a prefix they all share, read once for all, and
+    each sequence's own positions after it (gaje_hip_attention_prefix)."""
+    check(lib().gaje_hip_attention_prefix(q.ptr, ldq, cache, layer, prefix_table.ptr, prefix_len, n_head, scale,
+                                          out.ptr, ldo, workspace.ptr, workspace.nbytes, stream))
 
 
 def kwta(scores: DeviceBuffer, n: int, k: int, stream=None):

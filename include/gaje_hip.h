@@ -251,6 +251,114 @@ int gaje_hip_expf(const float *x, float *y, int64_t n, void *stream);
 int gaje_hip_attention(const float *q, const float *k_cache, const float *v_cache, int64_t seq_len,
                        int64_t capacity, int n_head, int n_head_kv, int head_dim, float *out, void *stream);
 
+/* ------------------------------------------ serving many sequences -------- */
+/* Attention over ragged prompts and over a KV cache in pages, the writes into
+ * that cache, and its pages' bookkeeping.  No reference counterpart (its cache
+ * is one Vec per sequence, nn/attention.rs:14-15,85-86, and it has neither
+ * batches nor matrix prefill); the softmax attention itself is
+ * GenomicAttention::forward_attention_core's (nn/attention.rs:87-127) with a
+ * caller-given scale and without its 1e-12, in another summation order.
+ *
+ * Element types of q, k, v, out and of a cache: one of these per call.  Scores,
+ * softmax statistics and sums are f32 whatever the type; for 16-bit types the
+ * softmax weights are rounded to the type before they meet the values. */
+enum { GAJE_DTYPE_F32 = 0, GAJE_DTYPE_F16 = 1, GAJE_DTYPE_BF16 = 2 };
+
+/* A paged KV cache, described by the caller's device buffers.  Pages hold
+ * `page` positions (a power of two, 8 to 1024) of every layer; sequence s has
+ * len[s] positions, position p in row p % page of page table[s][p / page].
+ * ref[i] counts the table entries that name page i (0: free).  head_dim is a
+ * multiple of 8 up to 256; k and v are 16-byte aligned.  No kernel follows a
+ * page id outside 0..n_pages-1: rows there read as zeros and are not written.
+ * len is taken as at most max_pages * page, and at least 0. */
+typedef struct {
+    void *k, *v;                 /* [n_layer][n_pages][page][n_head_kv][head_dim] of dtype */
+    int32_t *table;              /* [n_seq][max_pages] page ids, -1 past a sequence's last  */
+    int32_t *len;                /* [n_seq] cached positions                                */
+    int32_t *ref;                /* [n_pages] table entries that name a page                */
+    int64_t n_layer, n_pages, n_seq, max_pages;
+    int32_t dtype, page, n_head_kv, head_dim;
+} gaje_hip_kv_pages;
+
+/* Sequences forked, freed, cut and grown in one step.  Slot d becomes slot
+ * source[d] as it was before the call (source NULL: itself; -1: empty), its
+ * length then changed by add[d] (add NULL: 0; negative: the last positions are
+ * dropped).  Whole pages that are kept are shared; a page kept in part goes to
+ * the lowest slot that keeps part of it if no slot keeps it whole, and is
+ * copied (all layers, K and V) for every other one, so that no two slots write
+ * one page.  New pages are the lowest ones with ref 0 before the call, slots in
+ * ascending order; a page that this call frees can be taken by the next one.
+ * Results go to new_table [n_seq][max_pages] (-1 past the last page), new_len,
+ * new_ref, which must not overlap the cache's own arrays: the caller swaps
+ * them in.  status[0] (device) gets 0, or the sum of 1 (a source outside
+ * -1..n_seq-1), 2 (a length below 0 or past max_pages * page), 4 (too few free
+ * pages), 8 (a table entry in use outside the pool): then the new arrays are
+ * the old ones and no page is copied.  All arrays are device memory and nothing
+ * is read on the host, so that the call can be captured in a graph.
+ * `workspace`: gaje_hip_kv_workspace(c) bytes, 16-byte aligned; calls that share
+ * one must not overlap.  n_pages up to 2^26, n_seq up to 2^20. */
+int64_t gaje_hip_kv_workspace(const gaje_hip_kv_pages *c);
+int gaje_hip_kv_update(const gaje_hip_kv_pages *c, const int32_t *source, const int32_t *add, int32_t *new_table,
+                       int32_t *new_len, int32_t *new_ref, int32_t *status, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+
+/* The pages in use moved to the front of the pool: with L pages of ref > 0, the
+ * pages in use at L or above move, in ascending order, into the free ones below
+ * L, in ascending order (all layers, K and V, in place).  new_table and new_ref
+ * (not overlapping the cache's own) get the renamed entries and the moved
+ * counts, n_live[0] (device) gets L.  Entries outside the pool become -1. */
+int gaje_hip_kv_compact(const gaje_hip_kv_pages *c, int32_t *new_table, int32_t *new_ref, int32_t *n_live,
+                        void *workspace, int64_t workspace_bytes, void *stream);
+
+/* New K and V rows of one layer into the cache: rows seq_off[s]..seq_off[s+1]-1
+ * of k and v (T rows; ldk, ldv elements apart; head g of a row at
+ * g * head_dim) are the last positions of sequence s, whose length already
+ * counts them (gaje_hip_kv_update).  source_dtype is the rows' type: the cache's
+ * own, or f32 rounded to nearest even (NaN stays NaN).  seq_off: device
+ * [n_seq + 1], ascending.  Rows past seq_off[n_seq], and rows of a sequence that
+ * has more than its length, are not stored.  k, v 16-byte aligned, ldk and ldv
+ * multiples of 8. */
+int gaje_hip_kv_append(const gaje_hip_kv_pages *c, int64_t layer, int source_dtype, const void *k, int64_t ldk,
+                       const void *v, int64_t ldv, const int32_t *seq_off, int64_t T, void *stream);
+
+/* Causal GQA attention of several prompts whose rows stand one after another:
+ * sequence s is rows seq_off[s]..seq_off[s+1]-1 of q, k, v and out (T rows at
+ * most; ldq, ldk, ldv, ldo elements apart, so that q, k and v may be columns of
+ * one fused product), row i sees rows seq_off[s]..i.  Query head h reads K/V head
+ * h / (n_head / n_head_kv).  out row: softmax(scale q.k) v, written in the type.
+ * seq_off: device [n_seq + 1], ascending; empty sequences are allowed, rows past
+ * seq_off[n_seq] of out are left as they were.  NaN and infinities reach only the
+ * rows that see them.  head_dim a multiple of 8 up to 256, scale > 0 and finite,
+ * q, k, v, out 16-byte aligned with leading dimensions that are multiples of 8.
+ * `workspace`: the matching _workspace() bytes, 16-byte aligned; nothing is kept
+ * in it between calls, and calls that share one must not overlap. */
+int64_t gaje_hip_attention_packed_workspace(int64_t T, int64_t n_seq, int n_head, int n_head_kv, int head_dim);
+int gaje_hip_attention_packed(int dtype, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
+                              int64_t ldv, const int32_t *seq_off, int64_t n_seq, int64_t T, int n_head,
+                              int n_head_kv, int head_dim, float scale, void *out, int64_t ldo, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+
+/* The same attention over a paged cache (q and out of its dtype): rows
+ * seq_off[s]..seq_off[s+1]-1 are the last positions of sequence s (its length
+ * counts them, their K and V are in the pages), so that a row sees every cached
+ * position up to its own: one token per sequence, drafted tokens, a prompt's
+ * next chunk.  A row whose position would be negative sees nothing: zeros. */
+int64_t gaje_hip_attention_paged_workspace(const gaje_hip_kv_pages *c, int64_t T, int n_head);
+int gaje_hip_attention_paged(const void *q, int64_t ldq, const gaje_hip_kv_pages *c, int64_t layer,
+                             const int32_t *seq_off, int64_t T, int n_head, float scale, void *out, int64_t ldo,
+                             void *workspace, int64_t workspace_bytes, void *stream);
+
+/* One token of each of the cache's n_seq sequences (row s of q and out) where
+ * positions 0..prefix_len-1 hold the same K and V in all of them: those are read
+ * once, through prefix_table (device: the pages of prefix_len positions, such as
+ * one sequence's row of the table), for all sequences together, positions from
+ * prefix_len on through each sequence's own pages.  A sequence shorter than
+ * prefix_len sees that much of the prefix; one of length 0 gets zeros. */
+int64_t gaje_hip_attention_prefix_workspace(const gaje_hip_kv_pages *c, int64_t prefix_len, int n_head);
+int gaje_hip_attention_prefix(const void *q, int64_t ldq, const gaje_hip_kv_pages *c, int64_t layer,
+                              const int32_t *prefix_table, int64_t prefix_len, int n_head, float scale, void *out,
+                              int64_t ldo, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* lateral_inhibition_kwta (compute/kernels/lut.rs:45-61), in place. */
 int gaje_hip_kwta(float *scores, int64_t n, int64_t k, void *stream);
 
