@@ -73,6 +73,14 @@ int check_count(const char *what, int64_t n_seq, int64_t T) {
     return GAJE_OK;
 }
 
+// Rows times heads are counted in 32 bits.
+int check_attn_count(const char *what, int64_t n_seq, int64_t T, int n_head) {
+    GAJE_TRY(check_count(what, n_seq, T));
+    if (T * n_head > (int64_t)1 << 30)
+        return set_error(GAJE_ERR_UNSUPPORTED, "%s: %lld rows of %d heads (2^30 at most)", what, (long long)T, n_head);
+    return GAJE_OK;
+}
+
 int check_scale(const char *what, float scale) {
     if (!(scale > 0.0f) || !std::isfinite(scale))
         return set_error(GAJE_ERR_INVALID_ARG, "%s: scale %g (positive and finite)", what, (double)scale);
@@ -169,7 +177,7 @@ extern "C" int gaje_hip_kv_append(const gaje_hip_kv_pages *c, int64_t layer, int
 extern "C" int64_t gaje_hip_attention_packed_workspace(int64_t T, int64_t n_seq, int n_head, int n_head_kv,
                                                        int head_dim) {
     if (check_heads("attention_packed", GAJE_DTYPE_F32, n_head, n_head_kv, head_dim) != GAJE_OK ||
-        check_count("attention_packed", n_seq, T) != GAJE_OK)
+        check_attn_count("attention_packed", n_seq, T, n_head) != GAJE_OK)
         return -1;
     if (T == 0 || n_seq == 0) return 0;
     int64_t most = 0;  // a workspace serves every dtype
@@ -187,7 +195,7 @@ extern "C" int gaje_hip_attention_packed(int dtype, const void *q, int64_t ldq, 
     static const char *const me = "attention_packed";
     clear_error();
     GAJE_TRY(check_heads(me, dtype, n_head, n_head_kv, head_dim));
-    GAJE_TRY(check_count(me, n_seq, T));
+    GAJE_TRY(check_attn_count(me, n_seq, T, n_head));
     GAJE_TRY(check_scale(me, scale));
     if (T == 0 || n_seq == 0) return GAJE_OK;
     if (!seq_off) return set_error(GAJE_ERR_INVALID_ARG, "%s: null seq_off", me);
@@ -213,7 +221,7 @@ extern "C" int gaje_hip_attention_packed(int dtype, const void *q, int64_t ldq, 
 extern "C" int64_t gaje_hip_attention_paged_workspace(const gaje_hip_kv_pages *c, int64_t T, int n_head) {
     static const char *const me = "attention_paged";
     if (check_pages(me, c) != GAJE_OK || check_heads(me, c->dtype, n_head, c->n_head_kv, c->head_dim) != GAJE_OK ||
-        check_count(me, c->n_seq, T) != GAJE_OK)
+        check_attn_count(me, c->n_seq, T, n_head) != GAJE_OK)
         return -1;
     return T == 0 ? 0 : serve_attn_workspace(paged_params(c, 0, T, n_head));
 }
@@ -226,7 +234,7 @@ extern "C" int gaje_hip_attention_paged(const void *q, int64_t ldq, const gaje_h
     GAJE_TRY(check_pages(me, c));
     GAJE_TRY(check_layer(me, c, layer));
     GAJE_TRY(check_heads(me, c->dtype, n_head, c->n_head_kv, c->head_dim));
-    GAJE_TRY(check_count(me, c->n_seq, T));
+    GAJE_TRY(check_attn_count(me, c->n_seq, T, n_head));
     GAJE_TRY(check_scale(me, scale));
     if (T == 0) return GAJE_OK;
     if (!seq_off) return set_error(GAJE_ERR_INVALID_ARG, "%s: null seq_off", me);

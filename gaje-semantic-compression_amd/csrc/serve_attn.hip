@@ -8,7 +8,9 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "device_util.h"
@@ -19,8 +21,19 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) { return (float)v; }
+typedef float vf16 __attribute__((ext_vector_type(16)));
+typedef _Float16 vh8 __attribute__((ext_vector_type(8)));
+typedef __bf16 vb8 __attribute__((ext_vector_type(8)));
+
+// What a row outside the sequence, a padded dimension and a page outside the pool
+// read: loads are redirected here instead of being skipped.
+__device__ const vu4 zero_piece = {0, 0, 0, 0};
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
 
 // The rows of one sequence and its keys.
 struct Seq {
@@ -112,34 +125,879 @@ __device__ __forceinline__ int64_t seq_of_row(const ServeAttnParams &p, int64_t 
     return lo;
 }
 
+// ---- tiles ----
+// A workgroup of four waves takes a tile of up to 128 query rows of one K/V head: the
+// rows of a sequence are its (token, query head of the group) pairs, so that the heads
+// that share K and V read them together.  Wave w holds rows 32 w .. 32 w + 31, one per
+// lane pair (lane, lane + 32), and walks the keys in tiles of BN:
+//   S^T = K Q^T   A = 32 keys, B = 32 queries: lane l has query l % 32 and, per 32 keys,
+//                 keys 8 (i / 4) + 4 (l / 32) + i % 4 in registers i < 16
+//   O^T = V^T P^T the same registers, rounded to the type, are the B operand as they
+//                 stand if the keys of V^T's operand come in that order
+// so a row's maximum, sum and rescaling stay within two lanes, and the weights never
+// leave their registers.  K and V are staged in LDS in operand order (V transposed on
+// the way, 8 keys x 8 dimensions per thread with v_perm), so that every operand is one
+// conflict-free 16-byte read; two buffers, one barrier per tile, the next tile's global
+// loads in flight during a tile's products.  f32 runs the f32 matrix instructions (no
+// transposition: one key per half-wave and step).
+template <typename T, int HD>
+struct TileCfg {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int BN = F32 ? (HD == 64 ? 64 : 32) : 8192 / HD;  // keys per tile
+    static constexpr int EP = 16 / sizeof(T);                          // elements per 16-byte piece
+    static constexpr int PCS = HD / EP;                                // pieces per row
+    static constexpr int UNITS = BN / 8 * PCS;                         // of 8 rows x one piece, K or V
+    static constexpr int UPT = 2 * UNITS / 256;                        // units per thread
+    static constexpr int NT = HD / 32;                                 // 32-dimension blocks of O^T
+    static constexpr int TILE = BN * HD * (int)sizeof(T);              // bytes of K or V in LDS
+    static constexpr int LDS = 4 * TILE;
+    static constexpr int STEPS = HD / (F32 ? 8 : 16);                  // of the scores' operands
+};
+
+struct TilePlan {
+    int64_t tiles;   // bound on the tiles of a K/V head
+    int32_t bm;      // rows of a tile
+    int32_t splits;  // parts of the keys
+    int32_t part0;   // first partial result, -1: the whole result
+    int32_t least;   // keys a part has at least
+    int32_t key0;    // the first key (few rows only)
+};
+
+// Sequence and tile of workgroup b: sequence s has ceil(rows_s group / BM) tiles, the
+// ones over the longest contexts first.  Every wave scans the sequences for itself.
+__device__ __forceinline__ bool find_tile(const ServeAttnParams &p, int64_t b, int group, int BM, Seq &q, int64_t &tile) {
+    const int lane = threadIdx.x & 63;
+    if (!p.seq_off) {
+        const int64_t per = (group + BM - 1) / BM;
+        q = seq_at(p, b / per);
+        tile = b % per;
+        return b / per < p.n_seq;
+    }
+    int64_t base = 0;
+    for (int64_t s0 = 0; s0 < p.n_seq; s0 += WAVE) {
+        int64_t n = 0;
+        if (s0 + lane < p.n_seq) {
+            const int64_t r0 = min(max((int64_t)p.seq_off[s0 + lane], (int64_t)0), p.T);
+            n = max(min((int64_t)p.seq_off[s0 + lane + 1], p.T) - r0, (int64_t)0);
+        }
+        const int cnt = (int)((n * group + BM - 1) / BM);
+        int incl = cnt;
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const int x = __shfl_up(incl, o, WAVE);
+            if (lane >= o) incl += x;
+        }
+        const int total = __builtin_amdgcn_readlane(incl, WAVE - 1);
+        if (b < base + total) {
+            const uint64_t past = __ballot(base + incl > b);
+            const int l = __builtin_ctzll(past);
+            const int last = __builtin_amdgcn_readlane(incl, l), mine = __builtin_amdgcn_readlane(cnt, l);
+            tile = base + last - 1 - b;  // reversed: b = base + last - mine is the last tile
+            (void)mine;
+            q = seq_at(p, s0 + l);
+            return true;
+        }
+        base += total;
+    }
+    return false;
+}
+
+// Query row r of a tile's sequence (or, over a shared prefix, of all sequences): its
+// row of q and out, its head, the last key it sees (-1: none).
+struct Row {
+    int64_t t, lim;
+    int head;
+    bool valid;
+};
+template <bool PREFIX>
+__device__ __forceinline__ Row row_at(const ServeAttnParams &p, const Seq &q, int64_t r, int group, int g) {
+    Row w;
+    const int64_t tok = (uint32_t)r / (uint32_t)group;
+    w.head = g * group + (int)(r - tok * group);
+    if constexpr (PREFIX) {
+        w.valid = tok < p.n_seq;
+        w.t = w.valid ? tok : 0;
+        w.lim = min(min(max((int64_t)p.len[w.t], (int64_t)0), p.max_pages << p.page_shift), p.prefix_len) - 1;
+    } else {
+        w.valid = tok < q.rows;
+        w.t = q.row0 + (w.valid ? tok : 0);
+        w.lim = min(q.len - q.rows + tok, q.len - 1);
+    }
+    if (!w.valid) w.lim = -1;
+    return w;
+}
+
+// The keys of part `split` of [k0, k1): whole multiples of `unit`, at least `least`.
+__device__ __forceinline__ void part_of(int64_t k0, int64_t k1, int splits, int split, int least, int unit, int64_t &b, int64_t &e) {
+    int64_t size = max((k1 - k0 + splits - 1) / splits, (int64_t)least);
+    size = (size + unit - 1) / unit * unit;
+    b = min(k0 + split * size, k1);
+    e = min(b + size, k1);
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void attn_row_kernel(ServeAttnParams p) {
-    const int lane = threadIdx.x & 63, h = blockIdx.y;
+__device__ __forceinline__ void store_row(const ServeAttnParams &p, int64_t t, int head, int part, bool whole, bool seen, float m,
+                                          float l, const float (&o)[4]) {
+    const int lane = threadIdx.x & 63, hd = p.head_dim;
+    if (whole) {
+        T *out = (T *)p.out + t * p.ldo + (int64_t)head * hd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 64 * i < hd) out[lane + 64 * i] = (T)(seen ? o[i] / l : 0.0f);
+    } else {
+        const int64_t at = ((int64_t)part * p.T + t) * p.n_head + head;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 64 * i < hd) p.part_o[at * hd + lane + 64 * i] = o[i];
+        if (lane == 0) p.part_ml[at] = make_float2(m, l);
+    }
+}
+
+template <typename T, int HD, bool PREFIX>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(ServeAttnParams p, TilePlan plan) {
+    using C = TileCfg<T, HD>;
+    constexpr int BM = 128, BN = C::BN, NB = BN / 32;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5, l32 = lane & 31;
+    const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
+    Seq q{0, 0, 0, 0};
+    int64_t tile = blockIdx.x / p.n_head_kv;
+    if constexpr (!PREFIX) {
+        if (!find_tile(p, tile, group, BM, q, tile)) return;
+        q.row0 = uniform(q.row0), q.rows = uniform(q.rows), q.len = uniform(q.len), q.id = uniform(q.id);
+        tile = uniform(tile);
+    }
+    const bool whole = plan.part0 < 0;
+    const int part = plan.part0 + blockIdx.y;
+    const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
+    // the keys: up to the last row's last one
+    int64_t kend = PREFIX ? p.prefix_len : 0;
+    if constexpr (!PREFIX) {
+        const int64_t last = min(q.rows * group, (tile + 1) * BM) - 1;
+        kend = max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
+    }
+    int64_t kb0, kb1;
+    part_of(0, kend, plan.splits, blockIdx.y, plan.least, BN, kb0, kb1);
+    // this wave's rows: the largest and the smallest last key
+    int lim_hi = (int)row.lim, lim_lo = row.valid ? (int)row.lim : INT32_MAX;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lim_hi = max(lim_hi, __shfl_xor(lim_hi, o, WAVE));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, o, WAVE));
+    }
+    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+
+    // queries: B operand, piece 2 j + half of the row
+    vu4 qf[C::STEPS];
+    {
+        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
+#pragma unroll
+        for (int j = 0; j < C::STEPS; ++j) {
+            const int e = (2 * j + half) * C::EP;
+            qf[j] = *(row.valid && e < hd ? (const vu4 *)(Q + e) : &zero_piece);
+        }
+    }
+
+    // this thread's units: 8 rows x one piece of K or V
+    const T *Kg = (const T *)p.k + (int64_t)g * hd, *Vg = (const T *)p.v + (int64_t)g * hd;
+    vu4 rg[C::UPT][8];
+    int ids[C::UPT][2];
+    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + q.id * p.max_pages;
+    auto is_v = [&](int n) { return C::UPT == 2 ? n == 1 : wave >= 2; };
+    auto unit_of = [&](int n, int &pc, int &set) {
+        const int u = C::UPT == 2 ? tid : tid & 127;
+        pc = u % C::PCS;
+        set = u / C::PCS;
+    };
+    // key of row i of a unit: K in order; V (16-bit) in the order of the weights' registers
+    auto key_of = [&](bool v, int set, int i) {
+        if (C::F32 || !v) return set * 8 + i;
+        return (set >> 1) * 16 + (set & 1) * 4 + (i & 3) + (i >> 2) * 8;
+    };
+    auto load_ids = [&](int64_t k0) {
+        if (!p.table) return;
+#pragma unroll
+        for (int n = 0; n < C::UPT; ++n) {
+            int pc, set;
+            unit_of(n, pc, set);
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+                ids[n][a] = pages[min(k0 + key_of(is_v(n), set, 4 * a), kb1 - 1) >> p.page_shift];
+        }
+    };
+    auto load_tile = [&](int64_t k0) {
+#pragma unroll
+        for (int n = 0; n < C::UPT; ++n) {
+            int pc, set;
+            unit_of(n, pc, set);
+            const bool v = is_v(n), in = pc * C::EP < hd;
+            const T *base = (v ? Vg : Kg) + pc * C::EP;
+            const int64_t ld = v ? p.ldv : p.ldk;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t pos = k0 + key_of(v, set, i);
+                bool ok = in && pos < kb1;
+                int64_t slot = q.row0 + pos;
+                if (p.table) {
+                    const int id = ids[n][i >> 2];
+                    ok = ok && (uint32_t)id < (uint32_t)p.n_pages;
+                    slot = ((int64_t)id << p.page_shift) + (pos & (((int64_t)1 << p.page_shift) - 1));
+                }
+                rg[n][i] = *(ok ? (const vu4 *)(base + slot * ld) : &zero_piece);
+            }
+        }
+    };
+    auto store_tile = [&](int buf) {
+        char *Kl = lds + buf * 2 * C::TILE, *Vl = Kl + C::TILE;
+#pragma unroll
+        for (int n = 0; n < C::UPT; ++n) {
+            int pc, set;
+            unit_of(n, pc, set);
+            if (!is_v(n)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = set * 8 + i;
+                    *(vu4 *)(Kl + (((key >> 5) * C::STEPS + (pc >> 1)) * 64 + (pc & 1) * 32 + ((key & 31) ^ (pc & 31))) * 16) = rg[n][i];
+                }
+            } else if constexpr (C::F32) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) *(vu4 *)(Vl + ((set * 8 + i) * C::PCS + pc) * 16) = rg[n][i];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t a = rg[n][2 * k][e >> 1], b = rg[n][2 * k + 1][e >> 1];
+                        w[k] = __builtin_amdgcn_perm(b, a, e & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                    const int r = (e / C::NT) * C::PCS + pc;
+                    *(vu4 *)(Vl + (((set >> 1) * C::NT + e % C::NT) * 64 + (set & 1) * 32 + r) * 16) = vu4{w[0], w[1], w[2], w[3]};
+                }
+            }
+        }
+    };
+
+    const float c = p.scale * LOG2E;
+    float m = -INFINITY, l = 0.0f;
+    vf16 o[C::NT];
+#pragma unroll
+    for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+
+    if (kb0 < kb1) {
+        load_ids(kb0);
+        load_tile(kb0);
+        load_ids(kb0 + BN);
+        store_tile(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t k0 = kb0; k0 < kb1; k0 += BN, buf ^= 1) {
+        const bool more = k0 + BN < kb1;
+        if (more) {
+            load_tile(k0 + BN);
+            load_ids(k0 + 2 * BN);
+        }
+        if (k0 <= lim_hi) {
+            const char *Kl = lds + buf * 2 * C::TILE, *Vl = Kl + C::TILE;
+            vf16 s[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+            const int kx = ((l32 ^ half) << 4) + half * 512;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < C::STEPS; ++j) {
+                    const vu4 kf = *(const vu4 *)(Kl + (b * C::STEPS + j) * 1024 + (kx ^ ((2 * j & 31) << 4)));
+                    if constexpr (C::F32) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[i]), __uint_as_float(qf[j][i]), s[b], 0, 0, 0);
+                    } else if constexpr (sizeof(T) == 2 && std::is_same<T, _Float16>::value) {
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, kf), __builtin_bit_cast(vh8, qf[j]), s[b], 0, 0, 0);
+                    } else {
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, kf), __builtin_bit_cast(vb8, qf[j]), s[b], 0, 0, 0);
+                    }
+                }
+            if (k0 + BN - 1 > lim_lo) {
+                const int lim = (int)(row.lim - k0);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (b * 32 + 8 * (i >> 2) + 4 * half + (i & 3) > lim) s[b][i] = -INFINITY;
+            }
+            float mt = m;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[b][i]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+            const float base = mt == -INFINITY ? 0.0f : mt * c;
+            if (__any(mt != m)) {
+                const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m, c, -base));
+                l *= shrink;
+#pragma unroll
+                for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
+                m = mt;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -base));
+                    sum += s[b][i];
+                }
+            l += sum;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if constexpr (C::F32) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const char *vr = Vl + (b * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) * HD * 4;
+                        float vv[C::NT];
+                        if constexpr (C::NT == 2) {
+                            const float2 a = *(const float2 *)(vr + l32 * 8);
+                            vv[0] = a.x, vv[1] = a.y;
+                        } else {
+#pragma unroll
+                            for (int t = 0; t < C::NT; t += 4) {
+                                const float4 a = *(const float4 *)(vr + t * 128 + l32 * 16);
+                                vv[t] = a.x, vv[t + 1] = a.y, vv[t + 2] = a.z, vv[t + 3] = a.w;
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < C::NT; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv[t], s[b][i], o[t], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        T w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = (T)s[b][8 * st + i];
+#pragma unroll
+                        for (int t = 0; t < C::NT; ++t) {
+                            const vu4 vf = *(const vu4 *)(Vl + ((b * 2 + st) * C::NT + t) * 1024 + lane * 16);
+                            if constexpr (std::is_same<T, _Float16>::value)
+                                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, vf), __builtin_bit_cast(vh8, w), o[t], 0, 0, 0);
+                            else
+                                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, vf), __builtin_bit_cast(vb8, w), o[t], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        }
+        if (more) store_tile(buf ^ 1);
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32, WAVE);
+
+    // A row with a result that is no number: keys it does not see may be to blame (0 times
+    // NaN), so it is computed again key by key.
+    float odd = l * 0.0f;
+#pragma unroll
+    for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) odd = fmaf(o[t][i], 0.0f, odd);
+    odd += __shfl_xor(odd, 32, WAVE);
+    const bool again = row.valid && row.lim >= kb0 && kb0 < kb1 && odd != 0.0f;
+    uint32_t todo = (uint32_t)__ballot(again);
+
+    if (row.valid && !again) {
+        const bool seen = row.lim >= 0;
+        const int64_t at = ((int64_t)part * p.T + row.t) * p.n_head + row.head;
+        const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
+        T *out = (T *)p.out + row.t * p.ldo + (int64_t)row.head * hd;
+        float *po = p.part_o + at * hd;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = 8 * (i >> 2) + 4 * half + (i & 3);
+            // dimensions of row r of the blocks: NT (f32 of 256: twice 4) neighbours
+            constexpr int RUN = C::F32 && C::NT == 8 ? 4 : C::NT;
+#pragma unroll
+            for (int t0 = 0; t0 < C::NT; t0 += RUN) {
+                const int d = C::F32 ? t0 * 32 + r * RUN : (r % C::PCS) * 8 + (r / C::PCS) * C::NT;
+                if (d >= hd) continue;
+                if (whole) {
+                    T e[RUN];
+#pragma unroll
+                    for (int t = 0; t < RUN; ++t) e[t] = (T)(o[t0 + t][i] * inv);
+                    __builtin_memcpy(__builtin_assume_aligned(out + d, RUN * sizeof(T) > 16 ? 16 : RUN * sizeof(T)), e, sizeof e);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < RUN; ++t) po[d + t] = o[t0 + t][i];
+                }
+            }
+        }
+        if (!whole && half == 0) p.part_ml[at] = make_float2(m, l);
+    }
+    while (todo) {
+        const int n = __builtin_ctz(todo);
+        todo &= todo - 1;
+        const Row w = row_at<PREFIX>(p, q, tile * BM + wave * 32 + n, group, g);
+        const Seq qs = PREFIX ? seq_at(p, w.t) : q;
+        float mr, lr, orow[4];
+        attend_row<T>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
+        store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
+    }
+}
+
+// ---- few rows ----
+// A workgroup takes up to 16 NQ query rows of one K/V head (a decoded token's query heads,
+// a few drafted tokens), and its four waves take turns at the keys, KS each, every wave
+// with a softmax of its own until they are joined at the end.  Nothing is shared while the
+// keys stream by, so K and V go from memory to registers (two steps of them in flight)
+// and straight into the products:
+//   S^T = K Q^T   16 keys x 16 queries: lane l has query l % 16, keys 4 (l / 16) + i
+//   O^T = V^T P^T with those keys in that order; lane l reads HD / 16 neighbouring
+//                 dimensions of each key's row, of which the t-th belong to the t-th
+//                 16 x 16 block, transposed (16-bit types) with v_perm.
+// Bound by HBM: 2 hd elements per key against 4 hd operations per key and row.
+template <typename T, int HD>
+struct FewCfg {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int KB = F32 ? 1 : 2;              // blocks of 16 keys per step
+    static constexpr int KS = 16 * KB;                  // keys per step
+    static constexpr int EP = 16 / (int)sizeof(T);      // elements per piece
+    static constexpr int STEPS = HD / (4 * EP);         // K pieces of a lane per block
+    static constexpr int VW = HD / 16;                  // dimensions of a lane
+    static constexpr int VK = 4 * KB;                   // keys of a lane
+    static constexpr int VB = VW * (int)sizeof(T);      // bytes of a lane's row of V
+    static constexpr int VP = (VB + 15) / 16;           // pieces of it
+    static constexpr int NQ2 = HD == 256 ? 1 : 2;       // blocks of rows where there are more than 16
+};
+
+template <typename T, int HD, int NQ, bool PREFIX>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeAttnParams p, TilePlan plan) {
+    using C = FewCfg<T, HD>;
+    constexpr int BM = 16 * NQ;
+    __shared__ __align__(16) float joined[4][BM][HD];
+    __shared__ float ms[4][BM], ls[4][BM];
+    __shared__ int odd[BM];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, g4 = lane >> 4;
+    const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
+    Seq q{0, 0, 0, 0};
+    int64_t tile = blockIdx.x / p.n_head_kv;
+    if constexpr (!PREFIX) {
+        if (!find_tile(p, tile, group, BM, q, tile)) return;
+        q.row0 = uniform(q.row0), q.rows = uniform(q.rows), q.len = uniform(q.len), q.id = uniform(q.id);
+        tile = uniform(tile);
+    }
+    const bool whole = plan.part0 < 0;
+    const int part = plan.part0 + blockIdx.y;
+    int64_t kend = PREFIX ? p.prefix_len : 0;
+    if constexpr (!PREFIX) {
+        const int64_t last = min(q.rows * group, (tile + 1) * BM) - 1;
+        kend = max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
+    }
+    const int key0 = (int)min((int64_t)plan.key0, kend);
+    int64_t b64, e64;
+    part_of(key0 & ~31, kend, plan.splits, blockIdx.y, plan.least, 4 * C::KS, b64, e64);
+    const int kb0 = (int)b64, kb1 = (int)e64;
+    int lim[NQ], lim_hi = -1, lim_lo = INT32_MAX;
+    vu4 qf[NQ][C::STEPS];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const Row row = row_at<PREFIX>(p, q, tile * BM + n * 16 + l16, group, g);
+        lim[n] = (int)row.lim;
+        lim_hi = max(lim_hi, lim[n]);
+        if (row.valid) lim_lo = min(lim_lo, lim[n]);
+        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
+#pragma unroll
+        for (int j = 0; j < C::STEPS; ++j) {
+            const int e = (4 * j + g4) * C::EP;
+            qf[n][j] = *(row.valid && e < hd ? (const vu4 *)(Q + e) : &zero_piece);
+        }
+    }
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) {
+        lim_hi = max(lim_hi, __shfl_xor(lim_hi, x, WAVE));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, x, WAVE));
+    }
+    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+
+    const T *Kg = (const T *)p.k + (int64_t)g * hd, *Vg = (const T *)p.v + (int64_t)g * hd;
+    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + q.id * p.max_pages;
+    struct Step {
+        vu4 k[C::KB][C::STEPS];
+        vu4 v[C::VK][C::VP];
+    };
+    struct Ids {
+        int k[C::KB], v[C::KB];
+    };
+    auto load_ids = [&](Ids &d, int k0) {
+        if (!p.table) return;
+#pragma unroll
+        for (int b = 0; b < C::KB; ++b) {
+            d.k[b] = pages[min(k0 + b * 16 + l16, kb1 - 1) >> p.page_shift];
+            d.v[b] = pages[min(k0 + b * 16 + 4 * g4, kb1 - 1) >> p.page_shift];
+        }
+    };
+    auto slot_of = [&](int id, int pos, bool &ok) {
+        ok = ok && pos >= key0 && pos < kb1;
+        if (!p.table) return q.row0 + pos;
+        ok = ok && (uint32_t)id < (uint32_t)p.n_pages;
+        return ((int64_t)id << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+    };
+    auto load = [&](Step &x, const Ids &d, int k0) {
+#pragma unroll
+        for (int b = 0; b < C::KB; ++b) {
+            bool ok = true;
+            const T *kr = Kg + slot_of(d.k[b], k0 + b * 16 + l16, ok) * p.ldk;
+#pragma unroll
+            for (int j = 0; j < C::STEPS; ++j) {
+                const int e = (4 * j + g4) * C::EP;
+                x.k[b][j] = *(ok && e < hd ? (const vu4 *)(kr + e) : &zero_piece);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < C::VK; ++i) {
+            bool ok = true;
+            const T *vr = Vg + slot_of(d.v[i >> 2], k0 + (i >> 2) * 16 + 4 * g4 + (i & 3), ok) * p.ldv + l16 * C::VW;
+#pragma unroll
+            for (int j = 0; j < C::VP; ++j) {
+                const bool in = ok && l16 * C::VW + j * C::EP < hd;
+                if constexpr (C::VB == 8) {
+                    const vu2 h = *(in ? (const vu2 *)vr : (const vu2 *)&zero_piece);
+                    x.v[i][j] = vu4{h.x, h.y, 0, 0};
+                } else {
+                    x.v[i][j] = *(in ? (const vu4 *)(vr + j * C::EP) : &zero_piece);
+                }
+            }
+        }
+    };
+
+    const float c = p.scale * LOG2E;
+    float m[NQ], l[NQ];
+    vf4 o[NQ][C::VW];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        m[n] = -INFINITY, l[n] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < C::VW; ++t) o[n][t] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto compute = [&](const Step &x, int k0) {
+        vf4 s[NQ][C::KB];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int b = 0; b < C::KB; ++b) {
+                s[n][b] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < C::STEPS; ++j) {
+                    if constexpr (C::F32) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[b][j][i]), __uint_as_float(qf[n][j][i]), s[n][b], 0, 0, 0);
+                    } else if constexpr (std::is_same<T, _Float16>::value) {
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vh8, x.k[b][j]), __builtin_bit_cast(vh8, qf[n][j]), s[n][b], 0, 0, 0);
+                    } else {
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, x.k[b][j]), __builtin_bit_cast(vb8, qf[n][j]), s[n][b], 0, 0, 0);
+                    }
+                }
+            }
+        T w[NQ][8];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            if (k0 < key0 || k0 + C::KS - 1 > lim_lo) {
+#pragma unroll
+                for (int b = 0; b < C::KB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int pos = k0 + b * 16 + 4 * g4 + i;
+                        if (pos > lim[n] || pos < key0) s[n][b][i] = -INFINITY;
+                    }
+            }
+            float mt = m[n];
+#pragma unroll
+            for (int b = 0; b < C::KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[n][b][i]);
+            mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+            const float base = mt == -INFINITY ? 0.0f : mt * c;
+            if (__any(mt != m[n])) {
+                const float shrink = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m[n], c, -base));
+                l[n] *= shrink;
+#pragma unroll
+                for (int t = 0; t < C::VW; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[n][t][i] *= shrink;
+                m[n] = mt;
+            }
+#pragma unroll
+            for (int b = 0; b < C::KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[n][b][i] = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], c, -base));
+                    l[n] += s[n][b][i];
+                    w[n][4 * b + i] = (T)s[n][b][i];
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < C::VW; ++t) {
+            if constexpr (C::F32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[i][t >> 2][t & 3]), s[n][0][i], o[n][t], 0, 0, 0);
+            } else {
+                vu4 a;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    a[k] = __builtin_amdgcn_perm(x.v[2 * k + 1][t >> 3][(t & 7) >> 1], x.v[2 * k][t >> 3][(t & 7) >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    if constexpr (std::is_same<T, _Float16>::value)
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vh8, a), __builtin_bit_cast(vh8, w[n]), o[n][t], 0, 0, 0);
+                    else
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, w[n]), o[n][t], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    // two steps in flight, their page ids two more ahead
+    constexpr int STRIDE = 4 * C::KS;
+    int k0 = kb0 + wave * C::KS;
+    const int stop = min(kb1, lim_hi + 1);
+    if (k0 < stop) {
+        Step a, b;
+        Ids ia, ib;
+        load_ids(ia, k0);
+        load_ids(ib, k0 + STRIDE);
+        load(a, ia, k0);
+        for (; k0 < stop; k0 += 2 * STRIDE) {
+            load(b, ib, k0 + STRIDE);
+            load_ids(ia, k0 + 2 * STRIDE);
+            compute(a, k0);
+            if (k0 + STRIDE >= stop) break;
+            load(a, ia, k0 + 2 * STRIDE);
+            load_ids(ib, k0 + 3 * STRIDE);
+            compute(b, k0 + STRIDE);
+        }
+    }
+
+    // the four waves' results: each to the common maximum, then summed
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        l[n] += __shfl_xor(l[n], 16, WAVE);
+        l[n] += __shfl_xor(l[n], 32, WAVE);
+        if (g4 == 0) ms[wave][n * 16 + l16] = m[n], ls[wave][n * 16 + l16] = l[n];
+    }
+    if (tid < BM) odd[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ms[w][n * 16 + l16]);
+        const float base = mt == -INFINITY ? 0.0f : mt * c;
+        const float shrink = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m[n], c, -base));
+#pragma unroll
+        for (int t = 0; t < C::VW; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) joined[wave][n * 16 + l16][(4 * g4 + i) * C::VW + t] = m[n] == -INFINITY ? 0.0f : o[n][t][i] * shrink;
+    }
+    __syncthreads();
+    // 256 / BM threads per row
+    constexpr int TPR = 256 / BM, PER = HD / TPR;
+    const int r = tid / TPR, d0 = (tid % TPR) * 4;
+    const Row row = row_at<PREFIX>(p, q, tile * BM + r, group, g);
+    float mt = -INFINITY, lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ms[w][r]);
+    const float base = mt == -INFINITY ? 0.0f : mt * c;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        if (ms[w][r] != -INFINITY) lt = fmaf(ls[w][r], __builtin_amdgcn_exp2f(fmaf(ms[w][r], c, -base)), lt);
+        else lt += ls[w][r];
+    float4 v[PER / 4];
+    float bad = lt * 0.0f;
+#pragma unroll
+    for (int x = 0; x < PER / 4; ++x) {
+        const int d = d0 + x * TPR * 4;
+        v[x] = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float4 a = *(const float4 *)&joined[w][r][d];
+            v[x].x += a.x, v[x].y += a.y, v[x].z += a.z, v[x].w += a.w;
+        }
+        bad = fmaf(v[x].x, 0.0f, bad), bad = fmaf(v[x].y, 0.0f, bad), bad = fmaf(v[x].z, 0.0f, bad), bad = fmaf(v[x].w, 0.0f, bad);
+    }
+    // (as in the tiles: a row whose result is no number is computed again, key by key)
+    if (bad != 0.0f && row.valid && row.lim >= kb0 && kb0 < kb1) odd[r] = 1;
+    __syncthreads();
+    if (row.valid && !odd[r]) {
+        const bool seen = row.lim >= 0;
+        const int64_t at = ((int64_t)part * p.T + row.t) * p.n_head + row.head;
+        const float inv = whole ? (seen ? 1.0f / lt : 0.0f) : 1.0f;
+#pragma unroll
+        for (int x = 0; x < PER / 4; ++x) {
+            const int d = d0 + x * TPR * 4;
+            if (d >= hd) continue;
+            if (whole) {
+                T *out = (T *)p.out + row.t * p.ldo + (int64_t)row.head * hd + d;
+                T e[4] = {(T)(v[x].x * inv), (T)(v[x].y * inv), (T)(v[x].z * inv), (T)(v[x].w * inv)};
+                __builtin_memcpy(__builtin_assume_aligned(out, sizeof e), e, sizeof e);
+            } else {
+                *(float4 *)(p.part_o + at * hd + d) = v[x];
+            }
+        }
+        if (!whole && tid % TPR == 0) p.part_ml[at] = make_float2(mt, lt);
+    }
+    for (int n = wave; n < BM; n += 4) {
+        if (!odd[n]) continue;
+        const Row w = row_at<PREFIX>(p, q, tile * BM + n, group, g);
+        const Seq qs = PREFIX ? seq_at(p, w.t) : q;
+        float mr, lr, orow[4];
+        attend_row<T>(p, qs, w.t, w.head, max(kb0, key0), min((int64_t)kb1, w.lim + 1), mr, lr, orow);
+        store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
+    }
+}
+
+// ---- joining parts ----
+// One wave per (row, head): m = max_i m_i, o = sum_i 2^(c (m_i - m)) o_i over the same sum of l_i.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, int parts) {
+    const int lane = threadIdx.x & 63, hd = p.head_dim;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int h = blockIdx.y;
     if (t >= p.T) return;
     const int64_t s = seq_of_row(p, t);
     if (s < 0) return;
     const Seq q = seq_at(p, s);
-    const int64_t end = min(q.len - q.rows + (t - q.row0) + 1, q.len);
-    float m, l, o[4];
-    attend_row<T>(p, q, t, h, 0, end, m, l, o);
-    T *out = (T *)p.out + t * p.ldo + (int64_t)h * p.head_dim;
+    const bool seen = min(q.len - q.rows + (t - q.row0) + 1, q.len) > 0;
+    const float c = p.scale * LOG2E;
+    const int64_t step = p.T * p.n_head, at = t * p.n_head + h;
+    float m = -INFINITY;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[i * step + at].x);
+    const float base = m == -INFINITY ? 0.0f : m * c;
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < parts; ++i) {
+        const float2 ml = p.part_ml[i * step + at];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a part without keys
+        const float w = __builtin_amdgcn_exp2f(fmaf(ml.x, c, -base));
+        l = fmaf(w, ml.y, l);
+        const float *po = p.part_o + (i * step + at) * hd;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < p.head_dim) out[lane + 64 * i] = (T)(end > 0 ? o[i] / l : 0.0f);
+        for (int d = 0; d < 4; ++d)
+            if (lane + 64 * d < hd) o[d] = fmaf(w, po[lane + 64 * d], o[d]);
+    }
+    store_row<T>(p, t, h, 0, true, seen, m, l, o);
+}
+
+// ---- plans ----
+int hd_class(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+struct AttnPlan {
+    TilePlan keys, prefix;  // over the rows' own keys, and over the shared prefix
+    int parts;              // partial results to join, 0: none
+};
+
+// rows: query rows per K/V head of one sequence, as the host knows them (on average);
+// most: the keys a row can have.
+TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t most, int64_t key0) {
+    TilePlan t{};
+    const int64_t avg = rows / std::max<int64_t>(seqs, 1);
+    const int small = avg <= 16 || p.head_dim > 128 ? 16 : 32;
+    t.bm = avg <= small || key0 > 0 ? small : 128;  // (the tiles begin with key 0)
+    t.key0 = (int32_t)key0;
+    t.tiles = p.seq_off || !p.table ? rows / t.bm + std::min(seqs, p.T) : seqs * ((rows / seqs + t.bm - 1) / t.bm);
+    t.least = t.bm == 128 ? 256 : 128;
+    const int64_t blocks = std::max<int64_t>(t.tiles * p.n_head_kv, 1);
+    t.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(t.bm == 128 ? 512 : 1024) / blocks, (most + t.least - 1) / t.least, 64}));
+    return t;
+}
+
+AttnPlan make_plan(const ServeAttnParams &p) {
+    AttnPlan a{};
+    const int64_t group = p.n_head / p.n_head_kv, most = p.table ? p.max_pages << p.page_shift : p.T;
+    const int64_t first = p.prefix_table ? p.prefix_len : 0;
+    a.keys = plan_rows(p, p.n_seq, p.T * group, most - first, first);
+    a.keys.part0 = -1;
+    if (first > 0) {
+        a.prefix = plan_rows(p, 1, p.T * group, first, 0);
+        a.prefix.part0 = 0;
+        a.keys.part0 = a.prefix.splits;
+        a.parts = a.prefix.splits + a.keys.splits;
+    } else if (a.keys.splits > 1) {
+        a.keys.part0 = 0;
+        a.parts = a.keys.splits;
+    }
+    return a;
+}
+
+template <typename T, int HD, bool PREFIX>
+int launch_tiles(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
+    using C = TileCfg<T, HD>;
+    const int64_t blocks = plan.tiles * p.n_head_kv;
+    if (blocks > (int64_t)1 << 23)
+        return set_error(GAJE_ERR_UNSUPPORTED, "attention over %lld tiles of rows (2^23 at most)", (long long)blocks);
+    const dim3 grid((unsigned)blocks, (unsigned)plan.splits);
+    if (plan.bm == 16) {
+        attn_few_kernel<T, HD, 1, PREFIX><<<grid, 256, 0, s>>>(p, plan);
+    } else if (plan.bm == 32) {
+        attn_few_kernel<T, HD, FewCfg<T, HD>::NQ2, PREFIX><<<grid, 256, 0, s>>>(p, plan);
+    } else {
+        static std::atomic<bool> set[64];
+        int dev = 0;
+        GAJE_HIP_CHECK(hipGetDevice(&dev));
+        if (dev < 0 || dev >= 64 || !set[dev].load()) {
+            GAJE_HIP_CHECK(hipFuncSetAttribute((const void *)attn_tile_kernel<T, HD, PREFIX>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
+            if (dev >= 0 && dev < 64) set[dev].store(true);
+        }
+        attn_tile_kernel<T, HD, PREFIX><<<grid, 256, C::LDS, s>>>(p, plan);
+    }
+    GAJE_HIP_CHECK(hipGetLastError());
+    return GAJE_OK;
+}
+
+template <typename T, bool PREFIX>
+int launch_part(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
+    const int hd = hd_class(p.head_dim);
+    if (hd == 64) return launch_tiles<T, 64, PREFIX>(p, plan, s);
+    if (hd == 128) return launch_tiles<T, 128, PREFIX>(p, plan, s);
+    return launch_tiles<T, 256, PREFIX>(p, plan, s);
+}
+
+template <typename T>
+int launch_typed(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
+    if (a.prefix.tiles) GAJE_TRY((launch_part<T, true>(p, a.prefix, s)));
+    GAJE_TRY((launch_part<T, false>(p, a.keys, s)));
+    if (a.parts) {
+        attn_join_kernel<T><<<dim3((unsigned)((p.T + 3) / 4), (unsigned)p.n_head), 256, 0, s>>>(p, a.parts);
+        GAJE_HIP_CHECK(hipGetLastError());
+    }
+    return GAJE_OK;
 }
 
 }  // namespace
 
-int64_t serve_attn_workspace(const ServeAttnParams &) { return 0; }
+int64_t serve_attn_workspace(const ServeAttnParams &p) {
+    const int64_t n = make_plan(p).parts * p.T * p.n_head;
+    return n ? n * (8 + 4 * (int64_t)p.head_dim) + 16 : 0;
+}
 
-int launch_serve_attn(const ServeAttnParams &p, void *, hipStream_t s) {
-    const dim3 grid((unsigned)((p.T + 3) / 4), (unsigned)p.n_head);
-    if (p.dtype == GAJE_DTYPE_F32) attn_row_kernel<float><<<grid, 256, 0, s>>>(p);
-    else if (p.dtype == GAJE_DTYPE_F16) attn_row_kernel<_Float16><<<grid, 256, 0, s>>>(p);
-    else attn_row_kernel<__bf16><<<grid, 256, 0, s>>>(p);
-    GAJE_HIP_CHECK(hipGetLastError());
-    return GAJE_OK;
+int launch_serve_attn(const ServeAttnParams &params, void *workspace, hipStream_t s) {
+    ServeAttnParams p = params;
+    const AttnPlan a = make_plan(p);
+    if (!a.prefix.tiles) p.prefix_table = nullptr, p.prefix_len = 0;
+    p.part_ml = (float2 *)workspace;
+    p.part_o = (float *)workspace + ((2 * a.parts * p.T * p.n_head + 3) & ~(int64_t)3);
+    if (p.dtype == GAJE_DTYPE_F32) return launch_typed<float>(p, a, s);
+    if (p.dtype == GAJE_DTYPE_F16) return launch_typed<_Float16>(p, a, s);
+    return launch_typed<__bf16>(p, a, s);
 }
 
 }  // namespace gaje
