@@ -60,9 +60,9 @@ int check_layer(const char *what, const gaje_hip_kv_pages *c, int64_t layer) {
 // Rows of `width` elements, ld apart, read or written 16 bytes at a time.
 int check_rows(const char *what, const char *name, const void *p, int64_t ld, int64_t width) {
     if (!p) return set_error(GAJE_ERR_INVALID_ARG, "%s: null %s", what, name);
-    if (!aligned16(p) || ld % 8 || ld < width || ld > (int64_t)1 << 32)
+    if (!aligned16(p) || ld % 8 || ld < width || ld > (int64_t)1 << 21)
         return set_error(GAJE_ERR_INVALID_ARG,
-                         "%s: %s needs 16-byte aligned rows, a leading dimension of at least %lld and a multiple of 8 (got %lld)",
+                         "%s: %s needs 16-byte aligned rows, a leading dimension of %lld to 2^21 and a multiple of 8 (got %lld)",
                          what, name, (long long)width, (long long)ld);
     return GAJE_OK;
 }

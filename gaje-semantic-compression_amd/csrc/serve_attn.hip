@@ -28,6 +28,9 @@ typedef __bf16 vb8 __attribute__((ext_vector_type(8)));
 // What a row outside the sequence, a padded dimension and a page outside the pool
 // read: loads are redirected here instead of being skipped.
 __device__ const vu4 zero_piece = {0, 0, 0, 0};
+typedef const __attribute__((address_space(1))) vu4 *gvu4;
+typedef const __attribute__((address_space(1))) char *gchar;
+__device__ __forceinline__ gvu4 piece(const void *p, bool ok) { return ok ? (gvu4)(uintptr_t)p : (gvu4)(uintptr_t)&zero_piece; }
 
 __device__ __forceinline__ int64_t uniform(int64_t v) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
@@ -149,8 +152,9 @@ struct TileCfg {
     static constexpr int UNITS = BN / 8 * PCS;                         // of 8 rows x one piece, K or V
     static constexpr int UPT = 2 * UNITS / 256;                        // units per thread
     static constexpr int NT = HD / 32;                                 // 32-dimension blocks of O^T
-    static constexpr int TILE = BN * HD * (int)sizeof(T);              // bytes of K or V in LDS
-    static constexpr int LDS = 4 * TILE;
+    static constexpr int KROW = 32 * 16 + 16;                          // bytes of 32 keys' pieces in LDS, 4 banks on
+    static constexpr int KT = BN / 32 * PCS * KROW, VT = BN * HD * (int)sizeof(T);
+    static constexpr int LDS = 2 * (KT + VT);
     static constexpr int STEPS = HD / (F32 ? 8 : 16);                  // of the scores' operands
 };
 
@@ -277,8 +281,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         const int64_t last = min(q.rows * group, (tile + 1) * BM) - 1;
         kend = max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
     }
-    int64_t kb0, kb1;
-    part_of(0, kend, plan.splits, blockIdx.y, plan.least, BN, kb0, kb1);
+    int64_t b64, e64;
+    part_of(0, kend, plan.splits, blockIdx.y, plan.least, BN, b64, e64);
+    const int kb0 = (int)b64, kb1 = (int)e64;
     // this wave's rows: the largest and the smallest last key
     int lim_hi = (int)row.lim, lim_lo = row.valid ? (int)row.lim : INT32_MAX;
 #pragma unroll
@@ -295,91 +300,88 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
 #pragma unroll
         for (int j = 0; j < C::STEPS; ++j) {
             const int e = (2 * j + half) * C::EP;
-            qf[j] = *(row.valid && e < hd ? (const vu4 *)(Q + e) : &zero_piece);
+            qf[j] = *piece(Q + e, row.valid && e < hd);
         }
     }
 
-    // this thread's units: 8 rows x one piece of K or V
-    const T *Kg = (const T *)p.k + (int64_t)g * hd, *Vg = (const T *)p.v + (int64_t)g * hd;
+    // This thread's units: 8 rows x one piece of K or V, rows set * 8 + i (V of 16-bit types:
+    // in the order of the weights' registers), in two groups of four neighbours.
+    constexpr bool BOTH = C::UPT == 2;  // every thread has a unit of each
+    const int unit = BOTH ? tid : tid & 127, pc = unit % C::PCS, set = unit / C::PCS;
+    const bool in = pc * C::EP < hd;
+    auto is_v = [&](int n) { return BOTH ? n == 1 : wave >= 2; };
+    auto group_of = [&](bool v, int a) { return C::F32 || !v ? set * 8 + 4 * a : (set >> 1) * 16 + (set & 1) * 4 + 8 * a; };
     vu4 rg[C::UPT][8];
     int ids[C::UPT][2];
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + q.id * p.max_pages;
-    auto is_v = [&](int n) { return C::UPT == 2 ? n == 1 : wave >= 2; };
-    auto unit_of = [&](int n, int &pc, int &set) {
-        const int u = C::UPT == 2 ? tid : tid & 127;
-        pc = u % C::PCS;
-        set = u / C::PCS;
-    };
-    // key of row i of a unit: K in order; V (16-bit) in the order of the weights' registers
-    auto key_of = [&](bool v, int set, int i) {
-        if (C::F32 || !v) return set * 8 + i;
-        return (set >> 1) * 16 + (set & 1) * 4 + (i & 3) + (i >> 2) * 8;
-    };
-    auto load_ids = [&](int64_t k0) {
+    const int page_mask = (1 << p.page_shift) - 1;
+    auto load_ids = [&](int k0) {
         if (!p.table) return;
 #pragma unroll
-        for (int n = 0; n < C::UPT; ++n) {
-            int pc, set;
-            unit_of(n, pc, set);
+        for (int n = 0; n < C::UPT; ++n)
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
-                ids[n][a] = pages[min(k0 + key_of(is_v(n), set, 4 * a), kb1 - 1) >> p.page_shift];
-        }
+            for (int a = 0; a < 2; ++a) ids[n][a] = pages[min(k0 + group_of(is_v(n), a), kb1 - 1) >> p.page_shift];
     };
-    auto load_tile = [&](int64_t k0) {
+    auto load_tile = [&](int k0) {
 #pragma unroll
         for (int n = 0; n < C::UPT; ++n) {
-            int pc, set;
-            unit_of(n, pc, set);
-            const bool v = is_v(n), in = pc * C::EP < hd;
-            const T *base = (v ? Vg : Kg) + pc * C::EP;
-            const int64_t ld = v ? p.ldv : p.ldk;
+            const bool v = is_v(n);
+            const char *base = (const char *)((v ? (const T *)p.v : (const T *)p.k) + (int64_t)g * hd);
+            const uint32_t ld = (uint32_t)(v ? p.ldv : p.ldk) * sizeof(T);
+            const char *at[2];
+            bool held[2] = {true, true};
+            if (p.table) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int64_t pos = k0 + key_of(v, set, i);
-                bool ok = in && pos < kb1;
-                int64_t slot = q.row0 + pos;
-                if (p.table) {
-                    const int id = ids[n][i >> 2];
-                    ok = ok && (uint32_t)id < (uint32_t)p.n_pages;
-                    slot = ((int64_t)id << p.page_shift) + (pos & (((int64_t)1 << p.page_shift) - 1));
+                for (int a = 0; a < 2; ++a) {
+                    held[a] = (uint32_t)ids[n][a] < (uint32_t)p.n_pages;
+                    const uint32_t in_page = (uint32_t)((k0 + group_of(v, a)) & page_mask) * ld + pc * 16;
+                    at[a] = base + in_page + (uint64_t)(uint32_t)ids[n][a] * (ld << p.page_shift);
                 }
-                rg[n][i] = *(ok ? (const vu4 *)(base + slot * ld) : &zero_piece);
+            } else {
+                const char *tile0 = base + (q.row0 + k0) * (int64_t)ld;
+#pragma unroll
+                for (int a = 0; a < 2; ++a) at[a] = tile0 + (uint32_t)group_of(v, a) * ld + pc * 16;
+            }
+            if (k0 + BN <= kb1 && hd == HD && __all(held[0] & held[1])) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rg[n][i] = *(gvu4)(uintptr_t)(at[i >> 2] + (i & 3) * ld);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool ok = in & (k0 + group_of(v, i >> 2) + (i & 3) < kb1) & held[i >> 2];
+                    rg[n][i] = *piece(at[i >> 2] + (i & 3) * ld, ok);
+                }
             }
         }
     };
+    char *const Kw = lds + ((set >> 2) * C::PCS + pc) * C::KROW + (set & 3) * 128;
+    char *const Vw = lds + 2 * C::KT + (C::F32 ? (set * 8 * C::PCS + pc) * 16 : (set >> 1) * C::NT * 1024 + (set & 1) * 512 + pc * 16);
     auto store_tile = [&](int buf) {
-        char *Kl = lds + buf * 2 * C::TILE, *Vl = Kl + C::TILE;
 #pragma unroll
         for (int n = 0; n < C::UPT; ++n) {
-            int pc, set;
-            unit_of(n, pc, set);
             if (!is_v(n)) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = set * 8 + i;
-                    *(vu4 *)(Kl + (((key >> 5) * C::STEPS + (pc >> 1)) * 64 + (pc & 1) * 32 + ((key & 31) ^ (pc & 31))) * 16) = rg[n][i];
-                }
+                for (int i = 0; i < 8; ++i) *(vu4 *)(Kw + buf * C::KT + i * 16) = rg[n][i];
             } else if constexpr (C::F32) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) *(vu4 *)(Vl + ((set * 8 + i) * C::PCS + pc) * 16) = rg[n][i];
+                for (int i = 0; i < 8; ++i) *(vu4 *)(Vw + buf * C::VT + i * C::PCS * 16) = rg[n][i];
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    uint32_t w[4];
+                    vu4 w;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t a = rg[n][2 * k][e >> 1], b = rg[n][2 * k + 1][e >> 1];
-                        w[k] = __builtin_amdgcn_perm(b, a, e & 1 ? 0x07060302u : 0x05040100u);
-                    }
-                    const int r = (e / C::NT) * C::PCS + pc;
-                    *(vu4 *)(Vl + (((set >> 1) * C::NT + e % C::NT) * 64 + (set & 1) * 32 + r) * 16) = vu4{w[0], w[1], w[2], w[3]};
+                    for (int k = 0; k < 4; ++k)
+                        w[k] = __builtin_amdgcn_perm(rg[n][2 * k + 1][e >> 1], rg[n][2 * k][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                    *(vu4 *)(Vw + buf * C::VT + (e % C::NT) * 1024 + (e / C::NT) * C::PCS * 16) = w;
                 }
             }
         }
     };
 
     const float c = p.scale * LOG2E;
+    // The weights' base m follows the maximum only where that is past it by a factor of
+    // 2^8: they stay below 2^8, and O is seldom rescaled.
+    const float slack = 8.0f / c;
     float m = -INFINITY, l = 0.0f;
     vf16 o[C::NT];
 #pragma unroll
@@ -394,60 +396,62 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         store_tile(0);
     }
     __syncthreads();
+    const char *const Kr = lds + half * C::KROW + l32 * 16;
+    const char *const Vr = lds + 2 * C::KT + (C::F32 ? half * 4 * HD * 4 + l32 * (C::NT == 2 ? 8 : 16) : lane * 16);
     int buf = 0;
-    for (int64_t k0 = kb0; k0 < kb1; k0 += BN, buf ^= 1) {
+    for (int k0 = kb0; k0 < kb1; k0 += BN, buf ^= 1) {
         const bool more = k0 + BN < kb1;
         if (more) {
             load_tile(k0 + BN);
             load_ids(k0 + 2 * BN);
         }
         if (k0 <= lim_hi) {
-            const char *Kl = lds + buf * 2 * C::TILE, *Vl = Kl + C::TILE;
+            const char *Kl = Kr + buf * C::KT, *Vl = Vr + buf * C::VT;
             vf16 s[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-            const int kx = ((l32 ^ half) << 4) + half * 512;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int j = 0; j < C::STEPS; ++j) {
-                    const vu4 kf = *(const vu4 *)(Kl + (b * C::STEPS + j) * 1024 + (kx ^ ((2 * j & 31) << 4)));
+                    const vu4 kf = *(const vu4 *)(Kl + (b * C::PCS + 2 * j) * C::KROW);
                     if constexpr (C::F32) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[i]), __uint_as_float(qf[j][i]), s[b], 0, 0, 0);
-                    } else if constexpr (sizeof(T) == 2 && std::is_same<T, _Float16>::value) {
+                    } else if constexpr (std::is_same<T, _Float16>::value) {
                         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, kf), __builtin_bit_cast(vh8, qf[j]), s[b], 0, 0, 0);
                     } else {
                         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, kf), __builtin_bit_cast(vb8, qf[j]), s[b], 0, 0, 0);
                     }
                 }
+            }
             if (k0 + BN - 1 > lim_lo) {
-                const int lim = (int)(row.lim - k0);
+                int lim = (int)row.lim - k0 - 4 * half;
+                asm volatile("" : "+v"(lim));  // (keeps this a branch: most tiles are seen whole)
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (b * 32 + 8 * (i >> 2) + 4 * half + (i & 3) > lim) s[b][i] = -INFINITY;
+                        if (b * 32 + 8 * (i >> 2) + (i & 3) > lim) s[b][i] = -INFINITY;
             }
-            float mt = m;
+            float mt = s[0][0];
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[b][i]);
             mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-            const float base = mt == -INFINITY ? 0.0f : mt * c;
-            if (__any(mt != m)) {
-                const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m, c, -base));
+            if (__any(mt > m + slack)) {
+                const float to = fmaxf(mt, m);
+                const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - to) * c);
                 l *= shrink;
 #pragma unroll
                 for (int t = 0; t < C::NT; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
-                m = mt;
+                m = to;
             }
+            const float base = m == -INFINITY ? 0.0f : m * c;
             float sum = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -462,15 +466,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
                 if constexpr (C::F32) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const char *vr = Vl + (b * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) * HD * 4;
+                        const char *vr = Vl + (b * 32 + 8 * (i >> 2) + (i & 3)) * HD * 4;
                         float vv[C::NT];
                         if constexpr (C::NT == 2) {
-                            const float2 a = *(const float2 *)(vr + l32 * 8);
+                            const float2 a = *(const float2 *)vr;
                             vv[0] = a.x, vv[1] = a.y;
                         } else {
 #pragma unroll
                             for (int t = 0; t < C::NT; t += 4) {
-                                const float4 a = *(const float4 *)(vr + t * 128 + l32 * 16);
+                                const float4 a = *(const float4 *)(vr + t * 128);
                                 vv[t] = a.x, vv[t + 1] = a.y, vv[t + 2] = a.z, vv[t + 3] = a.w;
                             }
                         }
@@ -485,7 +489,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
                         for (int i = 0; i < 8; ++i) w[i] = (T)s[b][8 * st + i];
 #pragma unroll
                         for (int t = 0; t < C::NT; ++t) {
-                            const vu4 vf = *(const vu4 *)(Vl + ((b * 2 + st) * C::NT + t) * 1024 + lane * 16);
+                            const vu4 vf = *(const vu4 *)(Vl + ((b * 2 + st) * C::NT + t) * 1024);
                             if constexpr (std::is_same<T, _Float16>::value)
                                 o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, vf), __builtin_bit_cast(vh8, w), o[t], 0, 0, 0);
                             else
@@ -545,7 +549,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         const Row w = row_at<PREFIX>(p, q, tile * BM + wave * 32 + n, group, g);
         const Seq qs = PREFIX ? seq_at(p, w.t) : q;
         float mr, lr, orow[4];
-        attend_row<T>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
+        attend_row<T>(p, qs, w.t, w.head, kb0, min((int64_t)kb1, w.lim + 1), mr, lr, orow);
         store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
     }
 }
