@@ -163,7 +163,9 @@ struct TilePlan {
     int32_t bm;      // rows of a tile
     int32_t splits;  // parts of the keys
     int32_t part0;   // first partial result, -1: the whole result
+    int32_t alone;   // no other plan's parts join these: one part is the whole result
     int32_t least;   // keys a part has at least
+    int32_t unit;    // and a multiple of
     int32_t key0;    // the first key (few rows only)
 };
 
@@ -231,12 +233,19 @@ __device__ __forceinline__ Row row_at(const ServeAttnParams &p, const Seq &q, in
     return w;
 }
 
-// The keys of part `split` of [k0, k1): whole multiples of `unit`, at least `least`.
-__device__ __forceinline__ void part_of(int64_t k0, int64_t k1, int splits, int split, int least, int unit, int64_t &b, int64_t &e) {
-    int64_t size = max((k1 - k0 + splits - 1) / splits, (int64_t)least);
-    size = (size + unit - 1) / unit * unit;
-    b = min(k0 + split * size, k1);
-    e = min(b + size, k1);
+// Keys per part of [k0, k1): a multiple of `unit`, at least `least`, at most `splits` parts.
+__device__ __forceinline__ int part_size(int k0, int k1, int splits, int least, int unit) {
+    const int size = max((k1 - k0 + splits - 1) / splits, least);
+    return (size + unit - 1) / unit * unit;
+}
+
+// One past the last key that a tile's rows see; first and one past the last key that
+// its parts are cut from.
+template <bool PREFIX>
+__device__ __forceinline__ int tile_end(const ServeAttnParams &p, const Seq &q, int64_t tile, int bm, int group) {
+    if constexpr (PREFIX) return (int)p.prefix_len;
+    const int64_t last = min(q.rows * group, (tile + 1) * bm) - 1;
+    return (int)max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
 }
 
 template <typename T>
@@ -272,18 +281,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         q.row0 = uniform(q.row0), q.rows = uniform(q.rows), q.len = uniform(q.len), q.id = uniform(q.id);
         tile = uniform(tile);
     }
-    const bool whole = plan.part0 < 0;
-    const int part = plan.part0 + blockIdx.y;
+    const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
+    const int size = part_size(0, kend, plan.splits, plan.least, plan.unit);
+    const bool whole = plan.part0 < 0 || (plan.alone && size >= kend);
+    const int part = plan.part0 + blockIdx.y, kb0 = min((int)blockIdx.y * size, kend), kb1 = min(kb0 + size, kend);
+    if (blockIdx.y > 0 && kb0 >= kb1) return;
     const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
-    // the keys: up to the last row's last one
-    int64_t kend = PREFIX ? p.prefix_len : 0;
-    if constexpr (!PREFIX) {
-        const int64_t last = min(q.rows * group, (tile + 1) * BM) - 1;
-        kend = max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
-    }
-    int64_t b64, e64;
-    part_of(0, kend, plan.splits, blockIdx.y, plan.least, BN, b64, e64);
-    const int kb0 = (int)b64, kb1 = (int)e64;
     // this wave's rows: the largest and the smallest last key
     int lim_hi = (int)row.lim, lim_lo = row.valid ? (int)row.lim : INT32_MAX;
 #pragma unroll
@@ -596,17 +599,11 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
         q.row0 = uniform(q.row0), q.rows = uniform(q.rows), q.len = uniform(q.len), q.id = uniform(q.id);
         tile = uniform(tile);
     }
-    const bool whole = plan.part0 < 0;
-    const int part = plan.part0 + blockIdx.y;
-    int64_t kend = PREFIX ? p.prefix_len : 0;
-    if constexpr (!PREFIX) {
-        const int64_t last = min(q.rows * group, (tile + 1) * BM) - 1;
-        kend = max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
-    }
-    const int key0 = (int)min((int64_t)plan.key0, kend);
-    int64_t b64, e64;
-    part_of(key0 & ~31, kend, plan.splits, blockIdx.y, plan.least, 4 * C::KS, b64, e64);
-    const int kb0 = (int)b64, kb1 = (int)e64;
+    const int kend = tile_end<PREFIX>(p, q, tile, BM, group), key0 = min(plan.key0, kend), from = key0 & ~31;
+    const int size = part_size(from, kend, plan.splits, plan.least, plan.unit);
+    const bool whole = plan.part0 < 0 || (plan.alone && size >= kend - from);
+    const int part = plan.part0 + blockIdx.y, kb0 = min(from + (int)blockIdx.y * size, kend), kb1 = min(kb0 + size, kend);
+    if (blockIdx.y > 0 && kb0 >= kb1) return;
     int lim[NQ], lim_hi = -1, lim_lo = INT32_MAX;
     vu4 qf[NQ][C::STEPS];
 #pragma unroll
@@ -871,34 +868,59 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
 }
 
 // ---- joining parts ----
-// One wave per (row, head): m = max_i m_i, o = sum_i 2^(c (m_i - m)) o_i over the same sum of l_i.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, int parts) {
-    const int lane = threadIdx.x & 63, hd = p.head_dim;
+// One wave per (row, head): m = max_i m_i, o = sum_i 2^(c (m_i - m)) o_i over the same sum
+// of l_i, for rows whose keys were cut into parts.  Four dimensions per lane and 64 / LPP
+// parts side by side, LPP = the lanes of one row of parts; all loads of up to four such
+// rounds in flight.
+template <typename T, int LPP>
+__global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, TilePlan keys, TilePlan prefix) {
+    constexpr int SIDE = WAVE / LPP;
+    const int lane = threadIdx.x & 63, hd = p.head_dim, h = blockIdx.y, group = p.n_head / p.n_head_kv;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int h = blockIdx.y;
     if (t >= p.T) return;
     const int64_t s = seq_of_row(p, t);
     if (s < 0) return;
     const Seq q = seq_at(p, s);
+    // the parts that its tiles wrote
+    const int64_t tile = ((t - q.row0) * group + h % group) / keys.bm;
+    const int kend = tile_end<false>(p, q, tile, keys.bm, group), from = min(keys.key0, kend) & ~31;
+    const int size = part_size(from, kend, keys.splits, keys.least, keys.unit);
+    if (keys.alone && size >= kend - from) return;  // written whole
+    const int np = prefix.tiles ? ((int)p.prefix_len - 1) / part_size(0, (int)p.prefix_len, prefix.splits, prefix.least, prefix.unit) + 1 : 0;
+    const int parts = np + max((kend - from + size - 1) / size, 1);
     const bool seen = min(q.len - q.rows + (t - q.row0) + 1, q.len) > 0;
     const float c = p.scale * LOG2E;
     const int64_t step = p.T * p.n_head, at = t * p.n_head + h;
+    auto place = [&](int i) { return (i < np ? prefix.part0 + i : keys.part0 + i - np) * step + at; };
     float m = -INFINITY;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[i * step + at].x);
+    for (int i = lane; i < parts; i += WAVE) m = fmaxf(m, p.part_ml[place(i)].x);
+    m = wave_max(m);
     const float base = m == -INFINITY ? 0.0f : m * c;
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = p.part_ml[i * step + at];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a part without keys
-        const float w = __builtin_amdgcn_exp2f(fmaf(ml.x, c, -base));
+    float l = 0.0f;
+    vf4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int d = lane % LPP * 4;
+#pragma unroll 4
+    for (int i = lane / LPP; i < parts; i += SIDE) {
+        const float2 ml = p.part_ml[place(i)];
+        const vf4 po = *(const vf4 *)(p.part_o + place(i) * hd + min(d, hd - 4));
+        // (a part without a key that the row sees: -inf, 0)
+        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(ml.x, c, -base));
         l = fmaf(w, ml.y, l);
-        const float *po = p.part_o + (i * step + at) * hd;
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-            if (lane + 64 * d < hd) o[d] = fmaf(w, po[lane + 64 * d], o[d]);
+        for (int x = 0; x < 4; ++x) o[x] = fmaf(w, po[x], o[x]);
     }
-    store_row<T>(p, t, h, 0, true, seen, m, l, o);
+#pragma unroll
+    for (int x = LPP; x < WAVE; x <<= 1) {
+        l += __shfl_xor(l, x, WAVE);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) o[y] += __shfl_xor(o[y], x, WAVE);
+    }
+    if (lane < LPP && d < hd) {
+        T e[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) e[x] = (T)(seen ? o[x] / l : 0.0f);
+        __builtin_memcpy(__builtin_assume_aligned((T *)p.out + t * p.ldo + (int64_t)h * hd + d, sizeof e), e, sizeof e);
+    }
 }
 
 // ---- plans ----
@@ -919,8 +941,9 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     t.key0 = (int32_t)key0;
     t.tiles = p.seq_off || !p.table ? rows / t.bm + std::min(seqs, p.T) : seqs * ((rows / seqs + t.bm - 1) / t.bm);
     t.least = t.bm == 128 ? 256 : 128;
-    const int64_t blocks = std::max<int64_t>(t.tiles * p.n_head_kv, 1);
-    t.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(t.bm == 128 ? 512 : 1024) / blocks, (most + t.least - 1) / t.least, 64}));
+    t.unit = 128;
+    const int64_t blocks = std::max<int64_t>(t.tiles * p.n_head_kv, 1), want = t.bm == 128 ? 512 : 1024;
+    t.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + blocks - 1) / blocks, (most + t.least - 1) / t.least, 64}));
     return t;
 }
 
@@ -937,6 +960,7 @@ AttnPlan make_plan(const ServeAttnParams &p) {
         a.parts = a.prefix.splits + a.keys.splits;
     } else if (a.keys.splits > 1) {
         a.keys.part0 = 0;
+        a.keys.alone = 1;
         a.parts = a.keys.splits;
     }
     return a;
@@ -980,7 +1004,10 @@ int launch_typed(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
     if (a.prefix.tiles) GAJE_TRY((launch_part<T, true>(p, a.prefix, s)));
     GAJE_TRY((launch_part<T, false>(p, a.keys, s)));
     if (a.parts) {
-        attn_join_kernel<T><<<dim3((unsigned)((p.T + 3) / 4), (unsigned)p.n_head), 256, 0, s>>>(p, a.parts);
+        const dim3 grid((unsigned)((p.T + 3) / 4), (unsigned)p.n_head);
+        if (p.head_dim <= 64) attn_join_kernel<T, 16><<<grid, 256, 0, s>>>(p, a.keys, a.prefix);
+        else if (p.head_dim <= 128) attn_join_kernel<T, 32><<<grid, 256, 0, s>>>(p, a.keys, a.prefix);
+        else attn_join_kernel<T, 64><<<grid, 256, 0, s>>>(p, a.keys, a.prefix);
         GAJE_HIP_CHECK(hipGetLastError());
     }
     return GAJE_OK;
