@@ -616,7 +616,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
 #pragma unroll
         for (int j = 0; j < C::STEPS; ++j) {
             const int e = (4 * j + g4) * C::EP;
-            qf[n][j] = *(row.valid && e < hd ? (const vu4 *)(Q + e) : &zero_piece);
+            qf[n][j] = *piece(Q + e, row.valid && e < hd);
         }
     }
 #pragma unroll
@@ -626,8 +626,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     }
     lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
 
-    const T *Kg = (const T *)p.k + (int64_t)g * hd, *Vg = (const T *)p.v + (int64_t)g * hd;
+    const char *const Kg = (const char *)((const T *)p.k + (int64_t)g * hd), *const Vg = (const char *)((const T *)p.v + (int64_t)g * hd);
+    const uint32_t ldk = (uint32_t)p.ldk * sizeof(T), ldv = (uint32_t)p.ldv * sizeof(T);
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + q.id * p.max_pages;
+    const int page_mask = (1 << p.page_shift) - 1;
     struct Step {
         vu4 k[C::KB][C::STEPS];
         vu4 v[C::VK][C::VP];
@@ -643,41 +645,65 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
             d.v[b] = pages[min(k0 + b * 16 + 4 * g4, kb1 - 1) >> p.page_shift];
         }
     };
-    auto slot_of = [&](int id, int pos, bool &ok) {
-        ok = ok && pos >= key0 && pos < kb1;
-        if (!p.table) return q.row0 + pos;
-        ok = ok && (uint32_t)id < (uint32_t)p.n_pages;
-        return ((int64_t)id << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+    // the address of a position's row: one 64-bit product per group of rows of one page
+    auto row_of = [&](const char *base, uint32_t ld, int id, int pos) {
+        if (!p.table) return base + (q.row0 + pos) * (int64_t)ld;
+        return base + (uint32_t)(pos & page_mask) * ld + (uint64_t)(uint32_t)id * (ld << p.page_shift);
     };
     auto load = [&](Step &x, const Ids &d, int k0) {
+        bool held = true;
+        if (p.table) {
 #pragma unroll
-        for (int b = 0; b < C::KB; ++b) {
-            bool ok = true;
-            const T *kr = Kg + slot_of(d.k[b], k0 + b * 16 + l16, ok) * p.ldk;
+            for (int b = 0; b < C::KB; ++b) held = held & ((uint32_t)d.k[b] < (uint32_t)p.n_pages) & ((uint32_t)d.v[b] < (uint32_t)p.n_pages);
+        }
+        if (hd == HD && k0 >= key0 && k0 + C::KS <= kb1 && __all(held)) {
 #pragma unroll
-            for (int j = 0; j < C::STEPS; ++j) {
-                const int e = (4 * j + g4) * C::EP;
-                x.k[b][j] = *(ok && e < hd ? (const vu4 *)(kr + e) : &zero_piece);
+            for (int b = 0; b < C::KB; ++b) {
+                const char *kr = row_of(Kg, ldk, d.k[b], k0 + b * 16 + l16) + g4 * 16;
+                const char *vr = row_of(Vg, ldv, d.v[b], k0 + b * 16 + 4 * g4) + l16 * C::VB;
+#pragma unroll
+                for (int j = 0; j < C::STEPS; ++j) x.k[b][j] = *(gvu4)(uintptr_t)(kr + j * 64);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < C::VP; ++j) {
+                        const uintptr_t at = (uintptr_t)(vr + i * ldv + j * 16);
+                        if constexpr (C::VB == 8) {
+                            const vu2 h = *(const __attribute__((address_space(1))) vu2 *)at;
+                            x.v[4 * b + i][j] = vu4{h.x, h.y, 0, 0};
+                        } else {
+                            x.v[4 * b + i][j] = *(gvu4)at;
+                        }
+                    }
             }
+            return;
         }
 #pragma unroll
-        for (int i = 0; i < C::VK; ++i) {
-            bool ok = true;
-            const T *vr = Vg + slot_of(d.v[i >> 2], k0 + (i >> 2) * 16 + 4 * g4 + (i & 3), ok) * p.ldv + l16 * C::VW;
+        for (int b = 0; b < C::KB; ++b) {
+            const int kp = k0 + b * 16 + l16, vp = k0 + b * 16 + 4 * g4;
+            const bool kok = (kp >= key0) & (kp < kb1) & (!p.table | ((uint32_t)d.k[b] < (uint32_t)p.n_pages));
+            const bool vok = !p.table | ((uint32_t)d.v[b] < (uint32_t)p.n_pages);
+            const char *kr = row_of(Kg, ldk, d.k[b], kp) + g4 * 16, *vr = row_of(Vg, ldv, d.v[b], vp) + l16 * C::VB;
 #pragma unroll
-            for (int j = 0; j < C::VP; ++j) {
-                const bool in = ok && l16 * C::VW + j * C::EP < hd;
-                if constexpr (C::VB == 8) {
-                    const vu2 h = *(in ? (const vu2 *)vr : (const vu2 *)&zero_piece);
-                    x.v[i][j] = vu4{h.x, h.y, 0, 0};
-                } else {
-                    x.v[i][j] = *(in ? (const vu4 *)(vr + j * C::EP) : &zero_piece);
+            for (int j = 0; j < C::STEPS; ++j) x.k[b][j] = *piece(kr + j * 64, kok & ((4 * j + g4) * C::EP < hd));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool ok = vok & (vp + i >= key0) & (vp + i < kb1);
+#pragma unroll
+                for (int j = 0; j < C::VP; ++j) {
+                    const bool in = ok & (l16 * C::VW + j * C::EP < hd);
+                    if constexpr (C::VB == 8) {
+                        const vu2 h = *(const __attribute__((address_space(1))) vu2 *)piece(vr + i * ldv, in);
+                        x.v[4 * b + i][j] = vu4{h.x, h.y, 0, 0};
+                    } else {
+                        x.v[4 * b + i][j] = *piece(vr + i * ldv + j * 16, in);
+                    }
                 }
             }
         }
     };
 
-    const float c = p.scale * LOG2E;
+    const float c = p.scale * LOG2E, slack = 8.0f / c;  // (as in the tiles)
     float m[NQ], l[NQ];
     vf4 o[NQ][C::VW];
 #pragma unroll
@@ -718,16 +744,16 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
                         if (pos > lim[n] || pos < key0) s[n][b][i] = -INFINITY;
                     }
             }
-            float mt = m[n];
+            float mt = s[n][0][0];
 #pragma unroll
             for (int b = 0; b < C::KB; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[n][b][i]);
             mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
             mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-            const float base = mt == -INFINITY ? 0.0f : mt * c;
-            if (__any(mt != m[n])) {
-                const float shrink = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m[n], c, -base));
+            if (__any(mt > m[n] + slack)) {
+                mt = fmaxf(mt, m[n]);
+                const float shrink = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mt) * c);
                 l[n] *= shrink;
 #pragma unroll
                 for (int t = 0; t < C::VW; ++t)
@@ -735,6 +761,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
                     for (int i = 0; i < 4; ++i) o[n][t][i] *= shrink;
                 m[n] = mt;
             }
+            const float base = m[n] == -INFINITY ? 0.0f : m[n] * c;
 #pragma unroll
             for (int b = 0; b < C::KB; ++b)
 #pragma unroll
@@ -779,12 +806,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
         load_ids(ib, k0 + STRIDE);
         load(a, ia, k0);
         for (; k0 < stop; k0 += 2 * STRIDE) {
-            load(b, ib, k0 + STRIDE);
+            // (ids before rows: loads return in order, and a wait for an id must not be one for rows)
             load_ids(ia, k0 + 2 * STRIDE);
+            load(b, ib, k0 + STRIDE);
             compute(a, k0);
             if (k0 + STRIDE >= stop) break;
-            load(a, ia, k0 + 2 * STRIDE);
             load_ids(ib, k0 + 3 * STRIDE);
+            load(a, ia, k0 + 2 * STRIDE);
             compute(b, k0 + STRIDE);
         }
     }
