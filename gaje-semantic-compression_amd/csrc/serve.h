@@ -29,9 +29,11 @@ struct ServeAttnParams {
     int64_t max_pages, n_pages;
     int32_t page_shift;
     // shared prefix: positions 0..prefix_len-1 through prefix_table
+    // (one row per sequence, seq_off null)
     const int32_t *prefix_table;  // null: none
     int64_t prefix_len;
-    // partial results: [n_part][T][n_head] (maximum, sum) and [n_part][T][n_head][head_dim]
+    // keys per part, then partial results: [n_part][T][n_head] (maximum, sum) and [n_part][T][n_head][head_dim]
+    int32_t *part_size;
     float2 *part_ml;
     float *part_o;
 };

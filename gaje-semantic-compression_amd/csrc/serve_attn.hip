@@ -115,17 +115,21 @@ __device__ void attend_row(const ServeAttnParams &p, const Seq &q, int64_t t, in
     l_out = l;
 }
 
-// The sequence of row t, by the offsets (the last s with seq_off[s] <= t).
+// The sequence of row t, the last s with seq_off[s] <= t (-1: none), by the whole wave: 64
+// offsets a step.
 __device__ __forceinline__ int64_t seq_of_row(const ServeAttnParams &p, int64_t t) {
     if (!p.seq_off) return t;
-    if (t < p.seq_off[0] || t >= p.seq_off[p.n_seq]) return -1;
-    int64_t lo = 0, hi = p.n_seq;
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (p.seq_off[mid] <= t) lo = mid;
-        else hi = mid;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = (int)p.n_seq + 1;  // the offsets lo .. lo + n - 1 hold the last one <= t
+    while (n > 0) {
+        const int step = (n + WAVE - 1) / WAVE, i = lane * step;
+        const int count = __popcll(__ballot(i < n && p.seq_off[lo + i] <= t));
+        if (count == 0) return -1;
+        lo += (count - 1) * step;
+        n = min(step, n - (count - 1) * step);
+        if (step == 1) break;
     }
-    return lo;
+    return lo < p.n_seq ? lo : -1;
 }
 
 // ---- tiles ----
@@ -159,34 +163,87 @@ struct TileCfg {
 };
 
 struct TilePlan {
-    int64_t tiles;   // bound on the tiles of a K/V head
+    int64_t items;   // bound on the (tile, part) pairs of a K/V head
     int32_t bm;      // rows of a tile
-    int32_t splits;  // parts of the keys
-    int32_t part0;   // first partial result, -1: the whole result
-    int32_t alone;   // no other plan's parts join these: one part is the whole result
+    int32_t splits;  // parts that the keys of a tile have at most
+    int32_t part0;   // first partial result, -1: every tile has one part, the whole result
+    int32_t alone;   // no other plan's parts join these: a single part is the whole result
     int32_t least;   // keys a part has at least
-    int32_t unit;    // and a multiple of
     int32_t key0;    // the first key (few rows only)
+    int32_t target;  // (tile, part, K/V head) triples wanted
+    int32_t size;    // keys per part, 0: from the sequences' lengths, on the device
+};
+constexpr int PART_UNIT = 128;  // parts are whole multiples of it
+
+// Keys per part where `total` keys over all tiles are to make `target` parts and the longest
+// tile `splits` at most.
+__host__ __device__ __forceinline__ int part_size(int64_t total, int64_t longest, int splits, int least, int target) {
+    int64_t size = (total + target - 1) / target, floor = (longest + splits - 1) / splits;
+    size = size < floor ? floor : size;
+    size = size < least ? least : size;
+    return (int)((size + PART_UNIT - 1) / PART_UNIT * PART_UNIT);
+}
+
+// One past the last key that a tile's rows see.
+template <bool PREFIX>
+__device__ __forceinline__ int tile_end(const ServeAttnParams &p, const Seq &q, int64_t tile, int bm, int group) {
+    if constexpr (PREFIX) return (int)p.prefix_len;
+    const int64_t last = min(q.rows * group, (tile + 1) * bm) - 1;
+    return (int)max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
+}
+
+// What a workgroup does: part `part` of a tile's keys, `size` keys each.
+struct Item {
+    Seq q;
+    int64_t tile;
+    int part, size;
 };
 
-// Sequence and tile of workgroup b: sequence s has ceil(rows_s group / BM) tiles, the
-// ones over the longest contexts first.  Every wave scans the sequences for itself.
-__device__ __forceinline__ bool find_tile(const ServeAttnParams &p, int64_t b, int group, int BM, Seq &q, int64_t &tile) {
-    const int lane = threadIdx.x & 63;
-    if (!p.seq_off) {
-        const int64_t per = (group + BM - 1) / BM;
-        q = seq_at(p, b / per);
-        tile = b % per;
-        return b / per < p.n_seq;
+// Item b of a K/V head.  A sequence has ceil(rows group / bm) tiles, the ones over the
+// longest contexts first, and as many parts as its longest tile needs (a workgroup past a
+// shorter tile's end has nothing to do).  Every wave looks at all sequences, 64 at a time:
+// once for the part size, if the keys are cut at all, once for its item.
+template <bool PREFIX>
+__device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePlan &plan, int b, int group, Item &it) {
+    if constexpr (PREFIX) {
+        const int parts = ((int)p.prefix_len - 1) / plan.size + 1;
+        it.q = Seq{0, 0, 0, 0};
+        it.tile = b / parts;
+        it.part = b % parts;
+        it.size = plan.size;
+        return true;
     }
-    int64_t base = 0;
-    for (int64_t s0 = 0; s0 < p.n_seq; s0 += WAVE) {
-        int64_t n = 0;
-        if (s0 + lane < p.n_seq) {
-            const int64_t r0 = min(max((int64_t)p.seq_off[s0 + lane], (int64_t)0), p.T);
-            n = max(min((int64_t)p.seq_off[s0 + lane + 1], p.T) - r0, (int64_t)0);
+    const int lane = threadIdx.x & 63, from = plan.key0 & ~31;
+    int row0, rows, keys, tiles, cut;  // of sequence s0 + lane; cut: keys to cut into parts
+    auto look = [&](int64_t s0) {
+        const int64_t s = min(s0 + lane, p.n_seq - 1);
+        const Seq q = seq_at(p, s);
+        row0 = (int)q.row0;
+        rows = s0 + lane < p.n_seq ? (int)q.rows : 0;
+        keys = (int)q.len;
+        tiles = (int)(((int64_t)rows * group + plan.bm - 1) / plan.bm);
+        cut = max(keys - from, 0);
+    };
+    int size = plan.size;
+    if (size == 0) {
+        int64_t total = 0;
+        int longest = 0;
+        for (int64_t s0 = 0; s0 < p.n_seq; s0 += WAVE) {
+            look(s0);
+            // (a causal prompt's tiles see half of its own rows on average)
+            if (tiles) total += (int64_t)tiles * max(cut - rows / 2, cut / 2), longest = max(longest, cut);
         }
-        const int cnt = (int)((n * group + BM - 1) / BM);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            total += __shfl_xor(total, o, WAVE);
+            longest = max(longest, __shfl_xor(longest, o, WAVE));
+        }
+        size = __builtin_amdgcn_readfirstlane(part_size(total * p.n_head_kv, longest, plan.splits, plan.least, plan.target));
+    }
+    int base = 0;
+    for (int64_t s0 = 0; s0 < p.n_seq; s0 += WAVE) {
+        if (plan.size || p.n_seq > WAVE) look(s0);
+        const int parts = max((cut - 1) / size + 1, 1), cnt = tiles * parts;
         int incl = cnt;
 #pragma unroll
         for (int o = 1; o < WAVE; o <<= 1) {
@@ -195,12 +252,16 @@ __device__ __forceinline__ bool find_tile(const ServeAttnParams &p, int64_t b, i
         }
         const int total = __builtin_amdgcn_readlane(incl, WAVE - 1);
         if (b < base + total) {
-            const uint64_t past = __ballot(base + incl > b);
-            const int l = __builtin_ctzll(past);
-            const int last = __builtin_amdgcn_readlane(incl, l), mine = __builtin_amdgcn_readlane(cnt, l);
-            tile = base + last - 1 - b;  // reversed: b = base + last - mine is the last tile
-            (void)mine;
-            q = seq_at(p, s0 + l);
+            const int l = __builtin_ctzll(__ballot(base + incl > b));
+            const int n = __builtin_amdgcn_readlane(parts, l);
+            const int left = base + __builtin_amdgcn_readlane(incl, l) - 1 - b;  // items after this one
+            it.q.row0 = __builtin_amdgcn_readlane(row0, l);
+            it.q.rows = __builtin_amdgcn_readlane(rows, l);
+            it.q.len = __builtin_amdgcn_readlane(keys, l);
+            it.q.id = s0 + l;
+            it.tile = left / n;
+            it.part = n - 1 - left % n;
+            it.size = size;
             return true;
         }
         base += total;
@@ -233,21 +294,6 @@ __device__ __forceinline__ Row row_at(const ServeAttnParams &p, const Seq &q, in
     return w;
 }
 
-// Keys per part of [k0, k1): a multiple of `unit`, at least `least`, at most `splits` parts.
-__device__ __forceinline__ int part_size(int k0, int k1, int splits, int least, int unit) {
-    const int size = max((k1 - k0 + splits - 1) / splits, least);
-    return (size + unit - 1) / unit * unit;
-}
-
-// One past the last key that a tile's rows see; first and one past the last key that
-// its parts are cut from.
-template <bool PREFIX>
-__device__ __forceinline__ int tile_end(const ServeAttnParams &p, const Seq &q, int64_t tile, int bm, int group) {
-    if constexpr (PREFIX) return (int)p.prefix_len;
-    const int64_t last = min(q.rows * group, (tile + 1) * bm) - 1;
-    return (int)max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
-}
-
 template <typename T>
 __device__ __forceinline__ void store_row(const ServeAttnParams &p, int64_t t, int head, int part, bool whole, bool seen, float m,
                                           float l, const float (&o)[4]) {
@@ -274,18 +320,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, l32 = lane & 31;
     const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
-    Seq q{0, 0, 0, 0};
-    int64_t tile = blockIdx.x / p.n_head_kv;
-    if constexpr (!PREFIX) {
-        if (!find_tile(p, tile, group, BM, q, tile)) return;
-        q.row0 = uniform(q.row0), q.rows = uniform(q.rows), q.len = uniform(q.len), q.id = uniform(q.id);
-        tile = uniform(tile);
-    }
+    Item it;
+    if (!find_item<PREFIX>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
+    if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    const Seq q = it.q;
+    const int64_t tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
-    const int size = part_size(0, kend, plan.splits, plan.least, plan.unit);
-    const bool whole = plan.part0 < 0 || (plan.alone && size >= kend);
-    const int part = plan.part0 + blockIdx.y, kb0 = min((int)blockIdx.y * size, kend), kb1 = min(kb0 + size, kend);
-    if (blockIdx.y > 0 && kb0 >= kb1) return;
+    const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
+    const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
+    if (it.part > 0 && kb0 >= kb1) return;
     const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
     // this wave's rows: the largest and the smallest last key
     int lim_hi = (int)row.lim, lim_lo = row.valid ? (int)row.lim : INT32_MAX;
@@ -592,18 +635,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g4 = lane >> 4;
     const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
-    Seq q{0, 0, 0, 0};
-    int64_t tile = blockIdx.x / p.n_head_kv;
-    if constexpr (!PREFIX) {
-        if (!find_tile(p, tile, group, BM, q, tile)) return;
-        q.row0 = uniform(q.row0), q.rows = uniform(q.rows), q.len = uniform(q.len), q.id = uniform(q.id);
-        tile = uniform(tile);
-    }
+    Item it;
+    if (!find_item<PREFIX>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
+    if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    const Seq q = it.q;
+    const int64_t tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group), key0 = min(plan.key0, kend), from = key0 & ~31;
-    const int size = part_size(from, kend, plan.splits, plan.least, plan.unit);
-    const bool whole = plan.part0 < 0 || (plan.alone && size >= kend - from);
-    const int part = plan.part0 + blockIdx.y, kb0 = min(from + (int)blockIdx.y * size, kend), kb1 = min(kb0 + size, kend);
-    if (blockIdx.y > 0 && kb0 >= kb1) return;
+    const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend - from);
+    const int part = plan.part0 + it.part, kb0 = min(from + it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
+    if (it.part > 0 && kb0 >= kb1) return;
     int lim[NQ], lim_hi = -1, lim_lo = INT32_MAX;
     vu4 qf[NQ][C::STEPS];
 #pragma unroll
@@ -906,15 +946,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, TileP
     const int lane = threadIdx.x & 63, hd = p.head_dim, h = blockIdx.y, group = p.n_head / p.n_head_kv;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= p.T) return;
+    const int size = *p.part_size;
     const int64_t s = seq_of_row(p, t);
     if (s < 0) return;
     const Seq q = seq_at(p, s);
     // the parts that its tiles wrote
     const int64_t tile = ((t - q.row0) * group + h % group) / keys.bm;
     const int kend = tile_end<false>(p, q, tile, keys.bm, group), from = min(keys.key0, kend) & ~31;
-    const int size = part_size(from, kend, keys.splits, keys.least, keys.unit);
     if (keys.alone && size >= kend - from) return;  // written whole
-    const int np = prefix.tiles ? ((int)p.prefix_len - 1) / part_size(0, (int)p.prefix_len, prefix.splits, prefix.least, prefix.unit) + 1 : 0;
+    const int np = prefix.items ? ((int)p.prefix_len - 1) / prefix.size + 1 : 0;
     const int parts = np + max((kend - from + size - 1) / size, 1);
     const bool seen = min(q.len - q.rows + (t - q.row0) + 1, q.len) > 0;
     const float c = p.scale * LOG2E;
@@ -959,30 +999,39 @@ struct AttnPlan {
     int parts;              // partial results to join, 0: none
 };
 
-// rows: query rows per K/V head of one sequence, as the host knows them (on average);
-// most: the keys a row can have.
-TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t most, int64_t key0) {
+// seqs sequences of `rows` query rows per K/V head together, as the host knows them, whose
+// rows see up to `most` keys from key0 on.  prefix: all rows, the same keys.
+TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t most, int64_t key0, bool prefix) {
     TilePlan t{};
     const int64_t avg = rows / std::max<int64_t>(seqs, 1);
     const int small = avg <= 16 || p.head_dim > 128 ? 16 : 32;
     t.bm = avg <= small || key0 > 0 ? small : 128;  // (the tiles begin with key 0)
     t.key0 = (int32_t)key0;
-    t.tiles = p.seq_off || !p.table ? rows / t.bm + std::min(seqs, p.T) : seqs * ((rows / seqs + t.bm - 1) / t.bm);
     t.least = t.bm == 128 ? 256 : 128;
-    t.unit = 128;
-    const int64_t blocks = std::max<int64_t>(t.tiles * p.n_head_kv, 1), want = t.bm == 128 ? 512 : 1024;
-    t.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + blocks - 1) / blocks, (most + t.least - 1) / t.least, 64}));
+    t.target = 512;
+    // ragged sequences end in a tile that is not full
+    const int64_t tiles = prefix || p.prefix_table ? seqs * ((rows / seqs + t.bm - 1) / t.bm) : rows / t.bm + std::min(seqs, p.T);
+    const int64_t blocks = tiles * p.n_head_kv;
+    t.splits = blocks >= t.target ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(most + t.least - 1) / t.least, 16 * ((t.target + blocks - 1) / blocks), 64}));
+    // a sequence has at most keys / size + 1 parts per tile, and half of its keys count at least
+    t.items = tiles + (t.splits > 1 ? 2 * t.target / p.n_head_kv + 1 : 0);
+    if (t.splits == 1) t.size = INT32_MAX / 2;
+    if (prefix) {
+        t.size = part_size(most * blocks, most, t.splits, t.least, t.target);
+        t.splits = (int)((most - 1) / t.size + 1);
+        t.items = tiles * t.splits;
+    }
     return t;
 }
 
 AttnPlan make_plan(const ServeAttnParams &p) {
     AttnPlan a{};
     const int64_t group = p.n_head / p.n_head_kv, most = p.table ? p.max_pages << p.page_shift : p.T;
-    const int64_t first = p.prefix_table ? p.prefix_len : 0;
-    a.keys = plan_rows(p, p.n_seq, p.T * group, most - first, first);
+    const int64_t first = p.prefix_table ? p.prefix_len : 0;  // (set for single tokens only)
+    a.keys = plan_rows(p, p.n_seq, p.T * group, std::max<int64_t>(most - first, 1), first, false);
     a.keys.part0 = -1;
     if (first > 0) {
-        a.prefix = plan_rows(p, 1, p.T * group, first, 0);
+        a.prefix = plan_rows(p, 1, p.T * group, first, 0, true);
         a.prefix.part0 = 0;
         a.keys.part0 = a.prefix.splits;
         a.parts = a.prefix.splits + a.keys.splits;
@@ -997,10 +1046,10 @@ AttnPlan make_plan(const ServeAttnParams &p) {
 template <typename T, int HD, bool PREFIX>
 int launch_tiles(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
     using C = TileCfg<T, HD>;
-    const int64_t blocks = plan.tiles * p.n_head_kv;
+    const int64_t blocks = plan.items * p.n_head_kv;
     if (blocks > (int64_t)1 << 23)
         return set_error(GAJE_ERR_UNSUPPORTED, "attention over %lld tiles of rows (2^23 at most)", (long long)blocks);
-    const dim3 grid((unsigned)blocks, (unsigned)plan.splits);
+    const unsigned grid = (unsigned)blocks;
     if (plan.bm == 16) {
         attn_few_kernel<T, HD, 1, PREFIX><<<grid, 256, 0, s>>>(p, plan);
     } else if (plan.bm == 32) {
@@ -1029,7 +1078,7 @@ int launch_part(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
 
 template <typename T>
 int launch_typed(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
-    if (a.prefix.tiles) GAJE_TRY((launch_part<T, true>(p, a.prefix, s)));
+    if (a.prefix.items) GAJE_TRY((launch_part<T, true>(p, a.prefix, s)));
     GAJE_TRY((launch_part<T, false>(p, a.keys, s)));
     if (a.parts) {
         const dim3 grid((unsigned)((p.T + 3) / 4), (unsigned)p.n_head);
@@ -1045,15 +1094,16 @@ int launch_typed(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
 
 int64_t serve_attn_workspace(const ServeAttnParams &p) {
     const int64_t n = make_plan(p).parts * p.T * p.n_head;
-    return n ? n * (8 + 4 * (int64_t)p.head_dim) + 16 : 0;
+    return n ? n * (8 + 4 * (int64_t)p.head_dim) + 32 : 0;
 }
 
 int launch_serve_attn(const ServeAttnParams &params, void *workspace, hipStream_t s) {
     ServeAttnParams p = params;
     const AttnPlan a = make_plan(p);
-    if (!a.prefix.tiles) p.prefix_table = nullptr, p.prefix_len = 0;
-    p.part_ml = (float2 *)workspace;
-    p.part_o = (float *)workspace + ((2 * a.parts * p.T * p.n_head + 3) & ~(int64_t)3);
+    if (!a.prefix.items) p.prefix_table = nullptr, p.prefix_len = 0;
+    p.part_size = (int32_t *)workspace;
+    p.part_ml = (float2 *)workspace + 2;
+    p.part_o = (float *)workspace + 4 + ((2 * a.parts * p.T * p.n_head + 3) & ~(int64_t)3);
     if (p.dtype == GAJE_DTYPE_F32) return launch_typed<float>(p, a, s);
     if (p.dtype == GAJE_DTYPE_F16) return launch_typed<_Float16>(p, a, s);
     return launch_typed<__bf16>(p, a, s);
