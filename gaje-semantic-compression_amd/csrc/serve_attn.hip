@@ -32,38 +32,55 @@ typedef const __attribute__((address_space(1))) vu4 *gvu4;
 typedef const __attribute__((address_space(1))) char *gchar;
 __device__ __forceinline__ gvu4 piece(const void *p, bool ok) { return ok ? (gvu4)(uintptr_t)p : (gvu4)(uintptr_t)&zero_piece; }
 
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
-    return (int64_t)(((uint64_t)hi << 32) | lo);
+// Prefix sums (and running maxima of values >= 0) over the wave, by cross-lane moves
+// within the VALU.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int lane_move(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+    v += lane_move<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
+    v += lane_move<0x112, 0xf>(v);
+    v += lane_move<0x114, 0xf>(v);
+    v += lane_move<0x118, 0xf>(v);
+    v += lane_move<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+    v += lane_move<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ int wave_most(int v) {
+    v = max(v, lane_move<0x111, 0xf>(v));
+    v = max(v, lane_move<0x112, 0xf>(v));
+    v = max(v, lane_move<0x114, 0xf>(v));
+    v = max(v, lane_move<0x118, 0xf>(v));
+    v = max(v, lane_move<0x142, 0xa>(v));
+    v = max(v, lane_move<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, WAVE - 1);
 }
 
 // The rows of one sequence and its keys.
 struct Seq {
-    int64_t row0, rows;  // its rows of q and out
-    int64_t len;         // its keys
-    int64_t id;
+    int row0, rows;  // its rows of q and out
+    int len;         // its keys
+    int id;
 };
 
-__device__ __forceinline__ Seq seq_at(const ServeAttnParams &p, int64_t s) {
-    Seq q;
-    q.id = s;
+__device__ __forceinline__ int cached(const ServeAttnParams &p, int len) { return min(max(len, 0), (int)(p.max_pages << p.page_shift)); }
+
+__device__ __forceinline__ Seq seq_at(const ServeAttnParams &p, int s) {
+    Seq q{s, 1, 0, s};
+    const int len = p.table ? p.len[s] : 0;  // (all loads before the first use)
     if (p.seq_off) {
-        q.row0 = min(max((int64_t)p.seq_off[s], (int64_t)0), p.T);
-        q.rows = max(min((int64_t)p.seq_off[s + 1], p.T) - q.row0, (int64_t)0);
-    } else {
-        q.row0 = s;
-        q.rows = 1;
+        const int a = p.seq_off[s], b = p.seq_off[s + 1];
+        q.row0 = min(max(a, 0), (int)p.T);
+        q.rows = max(min(b, (int)p.T) - q.row0, 0);
     }
-    q.len = p.table ? min(max((int64_t)p.len[s], (int64_t)0), p.max_pages << p.page_shift) : q.rows;
+    q.len = p.table ? cached(p, len) : q.rows;
     return q;
 }
 
 // The row of k and v that holds a sequence's position, -1 where its page is outside
 // the pool.
 __device__ __forceinline__ int64_t slot_at(const ServeAttnParams &p, const Seq &q, int64_t pos) {
-    if (!p.table) return q.row0 + pos;
-    const int32_t *row = pos < p.prefix_len && p.prefix_table ? p.prefix_table : p.table + q.id * p.max_pages;
+    if (!p.table) return (int64_t)q.row0 + pos;
+    const int32_t *row = pos < p.prefix_len && p.prefix_table ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
     const int64_t id = row[pos >> p.page_shift];
     if (id < 0 || id >= p.n_pages) return -1;
     return (id << p.page_shift) + (pos & (((int64_t)1 << p.page_shift) - 1));
@@ -117,7 +134,7 @@ __device__ void attend_row(const ServeAttnParams &p, const Seq &q, int64_t t, in
 
 // The sequence of row t, the last s with seq_off[s] <= t (-1: none), by the whole wave: 64
 // offsets a step.
-__device__ __forceinline__ int64_t seq_of_row(const ServeAttnParams &p, int64_t t) {
+__device__ __forceinline__ int seq_of_row(const ServeAttnParams &p, int t) {
     if (!p.seq_off) return t;
     const int lane = threadIdx.x & 63;
     int lo = 0, n = (int)p.n_seq + 1;  // the offsets lo .. lo + n - 1 hold the last one <= t
@@ -170,33 +187,32 @@ struct TilePlan {
     int32_t alone;   // no other plan's parts join these: a single part is the whole result
     int32_t least;   // keys a part has at least
     int32_t key0;    // the first key (few rows only)
-    int32_t target;  // (tile, part, K/V head) triples wanted
+    int32_t blocks;  // log2 of the (tile, part, K/V head) triples wanted
     int32_t size;    // keys per part, 0: from the sequences' lengths, on the device
 };
 constexpr int PART_UNIT = 128;  // parts are whole multiples of it
 
-// Keys per part where `total` keys over all tiles are to make `target` parts and the longest
-// tile `splits` at most.
-__host__ __device__ __forceinline__ int part_size(int64_t total, int64_t longest, int splits, int least, int target) {
-    int64_t size = (total + target - 1) / target, floor = (longest + splits - 1) / splits;
-    size = size < floor ? floor : size;
-    size = size < least ? least : size;
-    return (int)((size + PART_UNIT - 1) / PART_UNIT * PART_UNIT);
+// Keys per part where `total` units of keys over all tiles and K/V heads are to make about
+// 2^blocks parts and the longest tile `splits` (a power of two) at most.
+__host__ __device__ __forceinline__ int part_size(int64_t total, int longest, int splits, int least, int blocks) {
+    const int64_t even = ((total >> blocks) + 1) * PART_UNIT;
+    const int floor = longest / splits + 1;
+    const int size = even > (1 << 30) ? 1 << 30 : (int)even;
+    return ((size < floor ? floor : size) < least ? least : (size < floor ? (floor + PART_UNIT - 1) / PART_UNIT * PART_UNIT : size));
 }
 
 // One past the last key that a tile's rows see.
 template <bool PREFIX>
-__device__ __forceinline__ int tile_end(const ServeAttnParams &p, const Seq &q, int64_t tile, int bm, int group) {
+__device__ __forceinline__ int tile_end(const ServeAttnParams &p, const Seq &q, int tile, int bm, int group) {
     if constexpr (PREFIX) return (int)p.prefix_len;
-    const int64_t last = min(q.rows * group, (tile + 1) * bm) - 1;
-    return (int)max(q.len - q.rows + (int64_t)((uint32_t)last / (uint32_t)group) + 1, (int64_t)0);
+    const uint32_t last = (uint32_t)min((int64_t)q.rows * group, (int64_t)(tile + 1) * bm) - 1;
+    return max(q.len - q.rows + (int)(last / (uint32_t)group) + 1, 0);
 }
 
 // What a workgroup does: part `part` of a tile's keys, `size` keys each.
 struct Item {
     Seq q;
-    int64_t tile;
-    int part, size;
+    int tile, part, size;
 };
 
 // Item b of a K/V head.  A sequence has ceil(rows group / bm) tiles, the ones over the
@@ -206,61 +222,49 @@ struct Item {
 template <bool PREFIX>
 __device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePlan &plan, int b, int group, Item &it) {
     if constexpr (PREFIX) {
-        const int parts = ((int)p.prefix_len - 1) / plan.size + 1;
         it.q = Seq{0, 0, 0, 0};
-        it.tile = b / parts;
-        it.part = b % parts;
+        it.tile = b / plan.splits;
+        it.part = b % plan.splits;
         it.size = plan.size;
         return true;
     }
-    const int lane = threadIdx.x & 63, from = plan.key0 & ~31;
-    int row0, rows, keys, tiles, cut;  // of sequence s0 + lane; cut: keys to cut into parts
-    auto look = [&](int64_t s0) {
-        const int64_t s = min(s0 + lane, p.n_seq - 1);
-        const Seq q = seq_at(p, s);
-        row0 = (int)q.row0;
-        rows = s0 + lane < p.n_seq ? (int)q.rows : 0;
-        keys = (int)q.len;
-        tiles = (int)(((int64_t)rows * group + plan.bm - 1) / plan.bm);
-        cut = max(keys - from, 0);
+    const int lane = threadIdx.x & 63, from = plan.key0 & ~31, n_seq = (int)p.n_seq, shift = __builtin_ctz(plan.bm);
+    Seq q;
+    int tiles, cut;  // of sequence s0 + lane; cut: keys to cut into parts
+    auto look = [&](int s0) {
+        q = seq_at(p, min(s0 + lane, n_seq - 1));
+        if (s0 + lane >= n_seq) q.rows = 0;
+        tiles = (int)(((int64_t)q.rows * group + plan.bm - 1) >> shift);
+        cut = max(q.len - from, 0);
     };
     int size = plan.size;
     if (size == 0) {
         int64_t total = 0;
         int longest = 0;
-        for (int64_t s0 = 0; s0 < p.n_seq; s0 += WAVE) {
+        for (int s0 = 0; s0 < n_seq; s0 += WAVE) {
             look(s0);
-            // (a causal prompt's tiles see half of its own rows on average)
-            if (tiles) total += (int64_t)tiles * max(cut - rows / 2, cut / 2), longest = max(longest, cut);
+            // (a causal prompt's tiles see half of its own rows on average; units of 128 keys)
+            const int units = tiles ? max(cut - q.rows / 2, cut / 2) / PART_UNIT + 1 : 0;
+            total += __builtin_amdgcn_readlane(wave_scan(tiles * units), WAVE - 1);
+            longest = max(longest, wave_most(tiles ? cut : 0));
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            total += __shfl_xor(total, o, WAVE);
-            longest = max(longest, __shfl_xor(longest, o, WAVE));
-        }
-        size = __builtin_amdgcn_readfirstlane(part_size(total * p.n_head_kv, longest, plan.splits, plan.least, plan.target));
+        size = part_size(total * p.n_head_kv, longest, plan.splits, plan.least, plan.blocks);
     }
     int base = 0;
-    for (int64_t s0 = 0; s0 < p.n_seq; s0 += WAVE) {
-        if (plan.size || p.n_seq > WAVE) look(s0);
-        const int parts = max((cut - 1) / size + 1, 1), cnt = tiles * parts;
-        int incl = cnt;
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const int x = __shfl_up(incl, o, WAVE);
-            if (lane >= o) incl += x;
-        }
-        const int total = __builtin_amdgcn_readlane(incl, WAVE - 1);
+    for (int s0 = 0; s0 < n_seq; s0 += WAVE) {
+        if (plan.size || n_seq > WAVE) look(s0);
+        const int parts = plan.splits == 1 ? 1 : (int)((uint32_t)max(cut - 1, 0) / (uint32_t)size) + 1;
+        const int incl = wave_scan(tiles * parts), total = __builtin_amdgcn_readlane(incl, WAVE - 1);
         if (b < base + total) {
             const int l = __builtin_ctzll(__ballot(base + incl > b));
             const int n = __builtin_amdgcn_readlane(parts, l);
             const int left = base + __builtin_amdgcn_readlane(incl, l) - 1 - b;  // items after this one
-            it.q.row0 = __builtin_amdgcn_readlane(row0, l);
-            it.q.rows = __builtin_amdgcn_readlane(rows, l);
-            it.q.len = __builtin_amdgcn_readlane(keys, l);
+            it.q.row0 = __builtin_amdgcn_readlane(q.row0, l);
+            it.q.rows = __builtin_amdgcn_readlane(q.rows, l);
+            it.q.len = __builtin_amdgcn_readlane(q.len, l);
             it.q.id = s0 + l;
-            it.tile = left / n;
-            it.part = n - 1 - left % n;
+            it.tile = (int)((uint32_t)left / (uint32_t)n);
+            it.part = n - 1 - (left - it.tile * n);
             it.size = size;
             return true;
         }
@@ -272,19 +276,19 @@ __device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePl
 // Query row r of a tile's sequence (or, over a shared prefix, of all sequences): its
 // row of q and out, its head, the last key it sees (-1: none).
 struct Row {
-    int64_t t, lim;
-    int head;
+    int64_t t;
+    int lim, head;
     bool valid;
 };
 template <bool PREFIX>
-__device__ __forceinline__ Row row_at(const ServeAttnParams &p, const Seq &q, int64_t r, int group, int g) {
+__device__ __forceinline__ Row row_at(const ServeAttnParams &p, const Seq &q, int r, int group, int g) {
     Row w;
-    const int64_t tok = (uint32_t)r / (uint32_t)group;
-    w.head = g * group + (int)(r - tok * group);
+    const int tok = (int)((uint32_t)r / (uint32_t)group);
+    w.head = g * group + (r - tok * group);
     if constexpr (PREFIX) {
         w.valid = tok < p.n_seq;
         w.t = w.valid ? tok : 0;
-        w.lim = min(min(max((int64_t)p.len[w.t], (int64_t)0), p.max_pages << p.page_shift), p.prefix_len) - 1;
+        w.lim = min(cached(p, p.len[w.t]), (int)p.prefix_len) - 1;
     } else {
         w.valid = tok < q.rows;
         w.t = q.row0 + (w.valid ? tok : 0);
@@ -324,14 +328,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     if (!find_item<PREFIX>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
     if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
-    const int64_t tile = it.tile;
+    const int tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
     const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
     if (it.part > 0 && kb0 >= kb1) return;
     const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
     // this wave's rows: the largest and the smallest last key
-    int lim_hi = (int)row.lim, lim_lo = row.valid ? (int)row.lim : INT32_MAX;
+    int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         lim_hi = max(lim_hi, __shfl_xor(lim_hi, o, WAVE));
@@ -359,7 +363,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     auto group_of = [&](bool v, int a) { return C::F32 || !v ? set * 8 + 4 * a : (set >> 1) * 16 + (set & 1) * 4 + 8 * a; };
     vu4 rg[C::UPT][8];
     int ids[C::UPT][2];
-    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + q.id * p.max_pages;
+    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
     const int page_mask = (1 << p.page_shift) - 1;
     auto load_ids = [&](int k0) {
         if (!p.table) return;
@@ -384,7 +388,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
                     at[a] = base + in_page + (uint64_t)(uint32_t)ids[n][a] * (ld << p.page_shift);
                 }
             } else {
-                const char *tile0 = base + (q.row0 + k0) * (int64_t)ld;
+                const char *tile0 = base + (int64_t)(q.row0 + k0) * ld;
 #pragma unroll
                 for (int a = 0; a < 2; ++a) at[a] = tile0 + (uint32_t)group_of(v, a) * ld + pc * 16;
             }
@@ -473,7 +477,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
                 }
             }
             if (k0 + BN - 1 > lim_lo) {
-                int lim = (int)row.lim - k0 - 4 * half;
+                int lim = row.lim - k0 - 4 * half;
                 asm volatile("" : "+v"(lim));  // (keeps this a branch: most tiles are seen whole)
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -593,9 +597,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         const int n = __builtin_ctz(todo);
         todo &= todo - 1;
         const Row w = row_at<PREFIX>(p, q, tile * BM + wave * 32 + n, group, g);
-        const Seq qs = PREFIX ? seq_at(p, w.t) : q;
+        const Seq qs = PREFIX ? seq_at(p, (int)w.t) : q;
         float mr, lr, orow[4];
-        attend_row<T>(p, qs, w.t, w.head, kb0, min((int64_t)kb1, w.lim + 1), mr, lr, orow);
+        attend_row<T>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
         store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
     }
 }
@@ -639,7 +643,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     if (!find_item<PREFIX>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
     if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
-    const int64_t tile = it.tile;
+    const int tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group), key0 = min(plan.key0, kend), from = key0 & ~31;
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend - from);
     const int part = plan.part0 + it.part, kb0 = min(from + it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
@@ -649,7 +653,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const Row row = row_at<PREFIX>(p, q, tile * BM + n * 16 + l16, group, g);
-        lim[n] = (int)row.lim;
+        lim[n] = row.lim;
         lim_hi = max(lim_hi, lim[n]);
         if (row.valid) lim_lo = min(lim_lo, lim[n]);
         const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
@@ -668,7 +672,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
 
     const char *const Kg = (const char *)((const T *)p.k + (int64_t)g * hd), *const Vg = (const char *)((const T *)p.v + (int64_t)g * hd);
     const uint32_t ldk = (uint32_t)p.ldk * sizeof(T), ldv = (uint32_t)p.ldv * sizeof(T);
-    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + q.id * p.max_pages;
+    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
     const int page_mask = (1 << p.page_shift) - 1;
     struct Step {
         vu4 k[C::KB][C::STEPS];
@@ -687,7 +691,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     };
     // the address of a position's row: one 64-bit product per group of rows of one page
     auto row_of = [&](const char *base, uint32_t ld, int id, int pos) {
-        if (!p.table) return base + (q.row0 + pos) * (int64_t)ld;
+        if (!p.table) return base + (int64_t)(q.row0 + pos) * ld;
         return base + (uint32_t)(pos & page_mask) * ld + (uint64_t)(uint32_t)id * (ld << p.page_shift);
     };
     auto load = [&](Step &x, const Ids &d, int k0) {
@@ -835,25 +839,24 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
         }
     };
 
-    // two steps in flight, their page ids two more ahead
+    // The next step in flight during a step's products, the page ids of the one after it ahead
+    // of that (loads return in order: a wait for an id must not be one for rows).  One copy of
+    // the code, for the instruction cache: HBM leaves time for the moves.
     constexpr int STRIDE = 4 * C::KS;
-    int k0 = kb0 + wave * C::KS;
-    const int stop = min(kb1, lim_hi + 1);
-    if (k0 < stop) {
-        Step a, b;
-        Ids ia, ib;
-        load_ids(ia, k0);
-        load_ids(ib, k0 + STRIDE);
-        load(a, ia, k0);
-        for (; k0 < stop; k0 += 2 * STRIDE) {
-            // (ids before rows: loads return in order, and a wait for an id must not be one for rows)
-            load_ids(ia, k0 + 2 * STRIDE);
-            load(b, ib, k0 + STRIDE);
-            compute(a, k0);
+    const int first = kb0 + wave * C::KS, stop = min(kb1, lim_hi + 1);
+    if (first < stop) {
+        Step now, next;
+        Ids ids;
+        load_ids(ids, first);
+        for (int k0 = first - STRIDE;; k0 += STRIDE) {
+            if (k0 + STRIDE < stop) {
+                const Ids held = ids;
+                load_ids(ids, k0 + 2 * STRIDE);
+                load(next, held, k0 + STRIDE);
+            }
+            if (k0 >= first) compute(now, k0);
             if (k0 + STRIDE >= stop) break;
-            load_ids(ib, k0 + 3 * STRIDE);
-            load(a, ia, k0 + 2 * STRIDE);
-            compute(b, k0 + STRIDE);
+            now = next;
         }
     }
 
@@ -928,9 +931,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     for (int n = wave; n < BM; n += 4) {
         if (!odd[n]) continue;
         const Row w = row_at<PREFIX>(p, q, tile * BM + n, group, g);
-        const Seq qs = PREFIX ? seq_at(p, w.t) : q;
+        const Seq qs = PREFIX ? seq_at(p, (int)w.t) : q;
         float mr, lr, orow[4];
-        attend_row<T>(p, qs, w.t, w.head, max(kb0, key0), min((int64_t)kb1, w.lim + 1), mr, lr, orow);
+        attend_row<T>(p, qs, w.t, w.head, max(kb0, key0), min(kb1, w.lim + 1), mr, lr, orow);
         store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
     }
 }
@@ -947,16 +950,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, TileP
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= p.T) return;
     const int size = *p.part_size;
-    const int64_t s = seq_of_row(p, t);
+    const int s = seq_of_row(p, (int)t);
     if (s < 0) return;
     const Seq q = seq_at(p, s);
     // the parts that its tiles wrote
-    const int64_t tile = ((t - q.row0) * group + h % group) / keys.bm;
+    const int tile = (int)((((int64_t)t - q.row0) * group + h % group) / keys.bm);
     const int kend = tile_end<false>(p, q, tile, keys.bm, group), from = min(keys.key0, kend) & ~31;
     if (keys.alone && size >= kend - from) return;  // written whole
-    const int np = prefix.items ? ((int)p.prefix_len - 1) / prefix.size + 1 : 0;
+    const int np = prefix.items ? prefix.splits : 0;
     const int parts = np + max((kend - from + size - 1) / size, 1);
-    const bool seen = min(q.len - q.rows + (t - q.row0) + 1, q.len) > 0;
+    const bool seen = min(q.len - q.rows + ((int)t - q.row0) + 1, q.len) > 0;
     const float c = p.scale * LOG2E;
     const int64_t step = p.T * p.n_head, at = t * p.n_head + h;
     auto place = [&](int i) { return (i < np ? prefix.part0 + i : keys.part0 + i - np) * step + at; };
@@ -1008,16 +1011,18 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     t.bm = avg <= small || key0 > 0 ? small : 128;  // (the tiles begin with key 0)
     t.key0 = (int32_t)key0;
     t.least = t.bm == 128 ? 256 : 128;
-    t.target = 512;
+    t.blocks = 9;
+    const int target = 1 << t.blocks;
     // ragged sequences end in a tile that is not full
     const int64_t tiles = prefix || p.prefix_table ? seqs * ((rows / seqs + t.bm - 1) / t.bm) : rows / t.bm + std::min(seqs, p.T);
     const int64_t blocks = tiles * p.n_head_kv;
-    t.splits = blocks >= t.target ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(most + t.least - 1) / t.least, 16 * ((t.target + blocks - 1) / blocks), 64}));
+    t.splits = 1;
+    while (blocks < target && t.splits < 64 && t.splits * blocks < 16 * target && t.splits * t.least < most) t.splits *= 2;
     // a sequence has at most keys / size + 1 parts per tile, and half of its keys count at least
-    t.items = tiles + (t.splits > 1 ? 2 * t.target / p.n_head_kv + 1 : 0);
+    t.items = tiles + (t.splits > 1 ? 2 * target / p.n_head_kv + 1 : 0);
     if (t.splits == 1) t.size = INT32_MAX / 2;
     if (prefix) {
-        t.size = part_size(most * blocks, most, t.splits, t.least, t.target);
+        t.size = part_size(most * blocks / PART_UNIT, (int)most, t.splits, t.least, t.blocks);
         t.splits = (int)((most - 1) / t.size + 1);
         t.items = tiles * t.splits;
     }

@@ -268,7 +268,8 @@ enum { GAJE_DTYPE_F32 = 0, GAJE_DTYPE_F16 = 1, GAJE_DTYPE_BF16 = 2 };
  * `page` positions (a power of two, 8 to 1024) of every layer; sequence s has
  * len[s] positions, position p in row p % page of page table[s][p / page].
  * ref[i] counts the table entries that name page i (0: free).  head_dim is a
- * multiple of 8 up to 256; k and v are 16-byte aligned.  No kernel follows a
+ * multiple of 8 up to 256; k and v are 16-byte aligned; max_pages * page is 2^24 at
+ * most.  No kernel follows a
  * page id outside 0..n_pages-1: rows there read as zeros and are not written.
  * len is taken as at most max_pages * page, and at least 0. */
 typedef struct {
