@@ -445,6 +445,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         load_ids(kb0 + BN);
         store_tile(0);
     }
+    // The queries are waited for here: in the loop that wait, repeated, would be one for the
+    // next tile's rows.
+#pragma unroll
+    for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[j]));
     __syncthreads();
     const char *const Kr = lds + half * C::KROW + l32 * 16;
     const char *const Vr = lds + 2 * C::KT + (C::F32 ? half * 4 * HD * 4 + l32 * (C::NT == 2 ? 8 : 16) : lane * 16);
@@ -848,6 +852,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
         Step now, next;
         Ids ids;
         load_ids(ids, first);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[n][j]));  // (waited for here, as in the tiles)
         for (int k0 = first - STRIDE;; k0 += STRIDE) {
             if (k0 + STRIDE < stop) {
                 const Ids held = ids;
