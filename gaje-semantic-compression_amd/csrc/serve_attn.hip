@@ -219,7 +219,10 @@ struct Item {
 // longest contexts first, and as many parts as its longest tile needs (a workgroup past a
 // shorter tile's end has nothing to do).  Every wave looks at all sequences, 64 at a time:
 // once for the part size, if the keys are cut at all, once for its item.
-template <bool PREFIX>
+// LONG_FIRST: of up to 64 sequences together, the items over the longest contexts first (an
+// item takes up to 70 us, and one begun last ends last: 24 prompts of up to 2000 tokens, 12 heads
+// of 128, bf16, 153 -> LONG_US us).
+template <bool PREFIX, bool LONG_FIRST>
 __device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePlan &plan, int b, int group, Item &it) {
     if constexpr (PREFIX) {
         it.q = Seq{0, 0, 0, 0};
@@ -254,11 +257,27 @@ __device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePl
     for (int s0 = 0; s0 < n_seq; s0 += WAVE) {
         if (plan.size || n_seq > WAVE) look(s0);
         const int parts = plan.splits == 1 ? 1 : (int)((uint32_t)max(cut - 1, 0) / (uint32_t)size) + 1;
-        const int incl = wave_scan(tiles * parts), total = __builtin_amdgcn_readlane(incl, WAVE - 1);
+        const int cnt = tiles * parts, incl = wave_scan(cnt), total = __builtin_amdgcn_readlane(incl, WAVE - 1);
         if (b < base + total) {
-            const int l = __builtin_ctzll(__ballot(base + incl > b));
+            int l, left;  // the sequence's lane, and its items after this one
+            if (LONG_FIRST && n_seq <= WAVE) {
+                // the largest depth with more than b items at it or deeper
+                int after = 0, most = wave_most(cnt);
+                left = 0;
+                while (most - left > 1) {
+                    const int mid = (left + most) >> 1;
+                    const int deeper = __builtin_amdgcn_readlane(wave_scan(max(cnt - mid, 0)), WAVE - 1);
+                    if (deeper > b) left = mid;
+                    else most = mid, after = deeper;
+                }
+                const uint64_t there = __ballot(cnt > left);
+                const int rank = __popcll(there & (((uint64_t)1 << lane) - 1));
+                l = __builtin_ctzll(__ballot(cnt > left && rank == b - after));
+            } else {
+                l = __builtin_ctzll(__ballot(base + incl > b));
+                left = base + __builtin_amdgcn_readlane(incl, l) - 1 - b;
+            }
             const int n = __builtin_amdgcn_readlane(parts, l);
-            const int left = base + __builtin_amdgcn_readlane(incl, l) - 1 - b;  // items after this one
             it.q.row0 = __builtin_amdgcn_readlane(q.row0, l);
             it.q.rows = __builtin_amdgcn_readlane(q.rows, l);
             it.q.len = __builtin_amdgcn_readlane(q.len, l);
@@ -325,7 +344,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     const int half = lane >> 5, l32 = lane & 31;
     const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
+    if (!find_item<PREFIX, true>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
     if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
     const int tile = it.tile;
@@ -463,11 +482,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
             const char *Kl = Kr + buf * C::KT, *Vl = Vr + buf * C::VT;
             vf16 s[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+            // (blocks in turn: no product waits for the one before it)
 #pragma unroll
-                for (int j = 0; j < C::STEPS; ++j) {
+            for (int j = 0; j < C::STEPS; ++j)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
                     const vu4 kf = *(const vu4 *)(Kl + (b * C::PCS + 2 * j) * C::KROW);
                     if constexpr (C::F32) {
 #pragma unroll
@@ -479,7 +501,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
                         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, kf), __builtin_bit_cast(vb8, qf[j]), s[b], 0, 0, 0);
                     }
                 }
-            }
             if (k0 + BN - 1 > lim_lo) {
                 int lim = row.lim - k0 - 4 * half;
                 asm volatile("" : "+v"(lim));  // (keeps this a branch: most tiles are seen whole)
@@ -644,7 +665,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     const int l16 = lane & 15, g4 = lane >> 4;
     const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
+    if (!find_item<PREFIX, false>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
     if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
     const int tile = it.tile;
