@@ -221,7 +221,7 @@ struct Item {
 // once for the part size, if the keys are cut at all, once for its item.
 // LONG_FIRST: of up to 64 sequences together, the items over the longest contexts first (an
 // item takes up to 70 us, and one begun last ends last: 24 prompts of up to 2000 tokens, 12 heads
-// of 128, bf16, 153 -> LONG_US us).
+// of 128, bf16, 153 -> 150 us).
 template <bool PREFIX, bool LONG_FIRST>
 __device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePlan &plan, int b, int group, Item &it) {
     if constexpr (PREFIX) {
@@ -626,6 +626,293 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         float mr, lr, orow[4];
         attend_row<T>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
         store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
+    }
+}
+
+// ---- f32 tiles ----
+// f32 rows on the bf16 matrix instructions: x = x0 + x1 + x2, each the next 8 bits of the
+// mantissa (cut, so that the three parts are exactly x), and x y summed from x0 y0, x0 y1,
+// x1 y0, x1 y1, x0 y2, x2 y0: what is left out is below 2^-22 of |x y|, about f32's own
+// rounding over a few products.  Six products at 16 times the rate of the f32 matrix
+// instructions; an infinity's parts are no numbers, and its rows are computed again.
+// A workgroup takes 64 rows of one K/V head, 16 a wave, and the keys 32 at a time:
+// S^T = K Q^T and O^T = V^T P^T in 16 x 16 blocks, lanes as in the few-row kernel.  K and V
+// are split on the way into LDS (operand order, V transposed); one buffer of 48 KB (128
+// dimensions), so that three workgroups of a CU fill each other's waits.
+template <int HD>
+struct SplitCfg {
+    static constexpr int BM = 64, BN = 32, PCS = HD / 8, STEPS = HD / 32, VT = HD / 16;
+    static constexpr int VD = HD / 64;                 // dimensions of V per thread
+    static constexpr int KU = BN * PCS / 256;          // rows x 8 dimensions of K per thread
+    static constexpr int KCH = 16 * 16 + 16;           // bytes of 16 keys' pieces, 4 banks on
+    static constexpr int KP = 2 * PCS * KCH, VP = VT * 1024;  // bytes of a plane
+    static constexpr int LDS = 3 * (KP + VP);
+};
+
+// The three parts of a and b, packed: a in the low halves.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
+    float x = a, y = b;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+        w[i] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+        if (i < 2) x -= __uint_as_float(u & 0xffff0000u), y -= __uint_as_float(v & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ vf4 mfma_bf16(vu4 a, vu4 b, vf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, b), c, 0, 0, 0);
+}
+
+template <int HD, bool PREFIX>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(ServeAttnParams p, TilePlan plan) {
+    using C = SplitCfg<HD>;
+    constexpr int BM = C::BM, BN = C::BN;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, g4 = lane >> 4;
+    const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
+    Item it;
+    if (!find_item<PREFIX, true>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
+    if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    const Seq q = it.q;
+    const int tile = it.tile;
+    const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
+    const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
+    const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
+    if (it.part > 0 && kb0 >= kb1) return;
+    const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 16 + l16, group, g);
+    int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) {
+        lim_hi = max(lim_hi, __shfl_xor(lim_hi, x, WAVE));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, x, WAVE));
+    }
+    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+
+    // K: rows tid / PCS (and 256 / PCS on), dimensions 8 (tid % PCS); V: dimensions VD (tid % 64) of
+    // the wave's eight keys 4 w + 0..3, 16 + 4 w + 0..3
+    const int kpc = tid % C::PCS, krow = tid / C::PCS, vd = lane * C::VD;
+    const char *const Kg = (const char *)((const float *)p.k + (int64_t)g * hd + kpc * 8);
+    const char *const Vg = (const char *)((const float *)p.v + (int64_t)g * hd + vd);
+    const uint32_t ldk = (uint32_t)p.ldk * 4, ldv = (uint32_t)p.ldv * 4;
+    const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
+    const int page_mask = (1 << p.page_shift) - 1;
+    vu4 kr[C::KU][2];
+    uint32_t vr[8][C::VD];
+    int kid[C::KU], vid[2];
+    auto load_ids = [&](int k0) {
+        if (!p.table) return;
+#pragma unroll
+        for (int n = 0; n < C::KU; ++n) kid[n] = pages[min(k0 + krow + n * (256 / C::PCS), kb1 - 1) >> p.page_shift];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) vid[a] = pages[min(k0 + 16 * a + 4 * wave, kb1 - 1) >> p.page_shift];
+    };
+    auto row_of = [&](const char *base, uint32_t ld, int id, int pos) {
+        if (!p.table) return base + (int64_t)(q.row0 + pos) * ld;
+        return base + (uint32_t)(pos & page_mask) * ld + (uint64_t)(uint32_t)id * (ld << p.page_shift);
+    };
+    auto load_tile = [&](int k0) {
+#pragma unroll
+        for (int n = 0; n < C::KU; ++n) {
+            const int pos = k0 + krow + n * (256 / C::PCS);
+            const bool ok = (pos < kb1) & (kpc * 8 < hd) & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
+            const char *at = row_of(Kg, ldk, kid[n], pos);
+            kr[n][0] = *piece(at, ok);
+            kr[n][1] = *piece(at + 16, ok);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int pos = k0 + (i >> 2) * 16 + 4 * wave + (i & 3);
+            const bool ok = (pos < kb1) & (vd < hd) & (!p.table | ((uint32_t)vid[i >> 2] < (uint32_t)p.n_pages));
+            const auto at = piece(row_of(Vg, ldv, vid[i >> 2], pos), ok);
+            if constexpr (C::VD == 4) {
+                const vu4 x = *at;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) vr[i][e] = x[e];
+            } else if constexpr (C::VD == 2) {
+                const vu2 x = *(const __attribute__((address_space(1))) vu2 *)at;
+                vr[i][0] = x.x, vr[i][1] = x.y;
+            } else {
+                vr[i][0] = *(const __attribute__((address_space(1))) uint32_t *)at;
+            }
+        }
+    };
+    char *const Kw = lds + ((krow >> 4) * C::PCS + kpc) * C::KCH + (krow & 15) * 16;
+    char *const Vw = lds + 3 * C::KP + (lane >> 4) * C::VD * 1024 + (wave * 16 + l16) * 16;
+    auto store_tile = [&]() {
+#pragma unroll
+        for (int n = 0; n < C::KU; ++n) {
+            vu4 w[3];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t u[3];
+                split3(__uint_as_float(kr[n][x >> 1][(x & 1) * 2]), __uint_as_float(kr[n][x >> 1][(x & 1) * 2 + 1]), u);
+                w[0][x] = u[0], w[1][x] = u[1], w[2][x] = u[2];
+            }
+            // (16 rows on where a block of keys has fewer threads)
+            char *to = Kw + (256 / C::PCS >= 16 ? n * (256 / C::PCS / 16) * C::PCS * C::KCH : (n & 1) * (256 / C::PCS) * 16 + (n >> 1) * C::PCS * C::KCH);
+#pragma unroll
+            for (int y = 0; y < 3; ++y) *(vu4 *)(to + y * C::KP) = w[y];
+        }
+#pragma unroll
+        for (int e = 0; e < C::VD; ++e) {
+            vu4 w[3];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t u[3];
+                split3(__uint_as_float(vr[2 * x][e]), __uint_as_float(vr[2 * x + 1][e]), u);
+                w[0][x] = u[0], w[1][x] = u[1], w[2][x] = u[2];
+            }
+#pragma unroll
+            for (int y = 0; y < 3; ++y) *(vu4 *)(Vw + e * 1024 + y * C::VP) = w[y];
+        }
+    };
+
+    vu4 qf[3][C::STEPS];
+    if (kb0 < kb1) {
+        load_ids(kb0);
+        load_tile(kb0);
+        load_ids(kb0 + BN);
+    }
+    {
+        const float *Q = (const float *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
+#pragma unroll
+        for (int j = 0; j < C::STEPS; ++j) {
+            const int e = (4 * j + g4) * 8;
+            const bool ok = row.valid && e < hd;
+            const vu4 a = *piece(Q + e, ok), b = *piece(Q + e + 4, ok);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t u[3];
+                const vu4 &h = x < 2 ? a : b;
+                split3(__uint_as_float(h[(x & 1) * 2]), __uint_as_float(h[(x & 1) * 2 + 1]), u);
+                qf[0][j][x] = u[0], qf[1][j][x] = u[1], qf[2][j][x] = u[2];
+            }
+        }
+    }
+    const float c = p.scale * LOG2E, slack = 8.0f / c;  // (as in the tiles)
+    float m = -INFINITY, l = 0.0f;
+    vf4 o[C::VT];
+#pragma unroll
+    for (int t = 0; t < C::VT; ++t) o[t] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+    const char *const Kr = lds + g4 * C::KCH + l16 * 16, *const Vr = lds + 3 * C::KP + lane * 16;
+    for (int k0 = kb0; k0 < kb1; k0 += BN) {
+        store_tile();
+        __syncthreads();
+        if (k0 + BN < kb1) {
+            load_tile(k0 + BN);
+            load_ids(k0 + 2 * BN);
+        }
+        if (k0 <= lim_hi) {
+            vf4 s[2] = {vf4{0.0f, 0.0f, 0.0f, 0.0f}, vf4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+            for (int j = 0; j < C::STEPS; ++j)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    vu4 k[3];
+#pragma unroll
+                    for (int y = 0; y < 3; ++y) k[y] = *(const vu4 *)(Kr + y * C::KP + (b * C::PCS + 4 * j) * C::KCH);
+                    s[b] = mfma_bf16(k[2], qf[0][j], s[b]);
+                    s[b] = mfma_bf16(k[1], qf[1][j], s[b]);
+                    s[b] = mfma_bf16(k[0], qf[2][j], s[b]);
+                    s[b] = mfma_bf16(k[1], qf[0][j], s[b]);
+                    s[b] = mfma_bf16(k[0], qf[1][j], s[b]);
+                    s[b] = mfma_bf16(k[0], qf[0][j], s[b]);
+                }
+            if (k0 + BN - 1 > lim_lo) {
+                int lim = row.lim - k0 - 4 * g4;
+                asm volatile("" : "+v"(lim));
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (b * 16 + i > lim) s[b][i] = -INFINITY;
+            }
+            float mt = s[0][0];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[b][i]);
+            mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+            if (__any(mt > m + slack)) {
+                const float to = fmaxf(mt, m);
+                const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - to) * c);
+                l *= shrink;
+#pragma unroll
+                for (int t = 0; t < C::VT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[t][i] *= shrink;
+                m = to;
+            }
+            const float base = m == -INFINITY ? 0.0f : m * c;
+            vu4 w[3];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -base)), e1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], c, -base));
+                    l += e0 + e1;
+                    uint32_t u[3];
+                    split3(e0, e1, u);
+                    w[0][b * 2 + i / 2] = u[0], w[1][b * 2 + i / 2] = u[1], w[2][b * 2 + i / 2] = u[2];
+                }
+#pragma unroll
+            for (int t = 0; t < C::VT; ++t) {
+                vu4 v[3];
+#pragma unroll
+                for (int y = 0; y < 3; ++y) v[y] = *(const vu4 *)(Vr + y * C::VP + t * 1024);
+                o[t] = mfma_bf16(v[2], w[0], o[t]);
+                o[t] = mfma_bf16(v[1], w[1], o[t]);
+                o[t] = mfma_bf16(v[0], w[2], o[t]);
+                o[t] = mfma_bf16(v[1], w[0], o[t]);
+                o[t] = mfma_bf16(v[0], w[1], o[t]);
+                o[t] = mfma_bf16(v[0], w[0], o[t]);
+            }
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+
+    // (as in the tiles: a row whose result is no number is computed again, key by key)
+    float odd = l * 0.0f;
+#pragma unroll
+    for (int t = 0; t < C::VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd = fmaf(o[t][i], 0.0f, odd);
+    odd += __shfl_xor(odd, 16, WAVE);
+    odd += __shfl_xor(odd, 32, WAVE);
+    const bool again = row.valid && row.lim >= kb0 && kb0 < kb1 && odd != 0.0f;
+    uint32_t todo = (uint32_t)__ballot(again) & 0xffffu;
+    if (row.valid && !again) {
+        const bool seen = row.lim >= 0;
+        const int64_t at = ((int64_t)part * p.T + row.t) * p.n_head + row.head;
+        const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
+        float *to = whole ? (float *)p.out + row.t * p.ldo + (int64_t)row.head * hd : p.part_o + at * hd;
+        // rows 4 g4 + i of blocks t0 .. t0 + VD - 1: 4 VD neighbouring dimensions
+#pragma unroll
+        for (int t0 = 0; t0 < C::VT; t0 += C::VD) {
+            const int d = C::VD * ((t0 / C::VD) * 16 + 4 * g4);
+            float e[4 * C::VD];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < C::VD; ++x) e[i * C::VD + x] = o[t0 + x][i] * inv;
+#pragma unroll
+            for (int x = 0; x < C::VD; ++x)
+                if (d + 4 * x < hd) *(vf4 *)(to + d + 4 * x) = vf4{e[4 * x], e[4 * x + 1], e[4 * x + 2], e[4 * x + 3]};
+        }
+        if (!whole && g4 == 0) p.part_ml[at] = make_float2(m, l);
+    }
+    while (todo) {
+        const int n = __builtin_ctz(todo);
+        todo &= todo - 1;
+        const Row w = row_at<PREFIX>(p, q, tile * BM + wave * 16 + n, group, g);
+        const Seq qs = PREFIX ? seq_at(p, (int)w.t) : q;
+        float mr, lr, orow[4];
+        attend_row<float>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
+        store_row<float>(p, w.t, w.head, part, whole, true, mr, lr, orow);
     }
 }
 
@@ -1037,9 +1324,10 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     TilePlan t{};
     const int64_t avg = rows / std::max<int64_t>(seqs, 1);
     const int small = avg <= 16 || p.head_dim > 128 ? 16 : 32;
-    t.bm = avg <= small || key0 > 0 ? small : 128;  // (the tiles begin with key 0)
+    const int large = p.dtype == GAJE_DTYPE_F32 ? 64 : 128;
+    t.bm = avg <= small || key0 > 0 ? small : large;  // (the tiles begin with key 0)
     t.key0 = (int32_t)key0;
-    t.least = t.bm == 128 ? 256 : 128;
+    t.least = t.bm >= 64 ? 256 : 128;
     t.blocks = 9;
     const int target = 1 << t.blocks;
     // ragged sequences end in a tile that is not full
@@ -1079,7 +1367,6 @@ AttnPlan make_plan(const ServeAttnParams &p) {
 
 template <typename T, int HD, bool PREFIX>
 int launch_tiles(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
-    using C = TileCfg<T, HD>;
     const int64_t blocks = plan.items * p.n_head_kv;
     if (blocks > (int64_t)1 << 23)
         return set_error(GAJE_ERR_UNSUPPORTED, "attention over %lld tiles of rows (2^23 at most)", (long long)blocks);
@@ -1089,14 +1376,24 @@ int launch_tiles(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) 
     } else if (plan.bm == 32) {
         attn_few_kernel<T, HD, FewCfg<T, HD>::NQ2, PREFIX><<<grid, 256, 0, s>>>(p, plan);
     } else {
+        const void *kernel;
+        size_t lds;
+        if constexpr (sizeof(T) == 4) {
+            kernel = (const void *)attn_split_kernel<HD, PREFIX>;
+            lds = SplitCfg<HD>::LDS;
+        } else {
+            kernel = (const void *)attn_tile_kernel<T, HD, PREFIX>;
+            lds = TileCfg<T, HD>::LDS;
+        }
         static std::atomic<bool> set[64];
         int dev = 0;
         GAJE_HIP_CHECK(hipGetDevice(&dev));
         if (dev < 0 || dev >= 64 || !set[dev].load()) {
-            GAJE_HIP_CHECK(hipFuncSetAttribute((const void *)attn_tile_kernel<T, HD, PREFIX>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
+            GAJE_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
             if (dev >= 0 && dev < 64) set[dev].store(true);
         }
-        attn_tile_kernel<T, HD, PREFIX><<<grid, 256, C::LDS, s>>>(p, plan);
+        if constexpr (sizeof(T) == 4) attn_split_kernel<HD, PREFIX><<<grid, 256, lds, s>>>(p, plan);
+        else attn_tile_kernel<T, HD, PREFIX><<<grid, 256, lds, s>>>(p, plan);
     }
     GAJE_HIP_CHECK(hipGetLastError());
     return GAJE_OK;
