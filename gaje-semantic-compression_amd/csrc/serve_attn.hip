@@ -659,6 +659,8 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
         if (i < 2) x -= __uint_as_float(u & 0xffff0000u), y -= __uint_as_float(v & 0xffff0000u);
     }
 }
+// the products, the smallest first
+constexpr int SPLIT_A[6] = {2, 1, 0, 1, 0, 0}, SPLIT_B[6] = {0, 1, 2, 0, 1, 0};
 __device__ __forceinline__ vf4 mfma_bf16(vu4 a, vu4 b, vf4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, b), c, 0, 0, 0);
 }
@@ -711,31 +713,48 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
         if (!p.table) return base + (int64_t)(q.row0 + pos) * ld;
         return base + (uint32_t)(pos & page_mask) * ld + (uint64_t)(uint32_t)id * (ld << p.page_shift);
     };
+    auto take_v = [&](uint32_t (&to)[C::VD], gvu4 at) {
+        if constexpr (C::VD == 4) {
+            const vu4 x = *at;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e] = x[e];
+        } else if constexpr (C::VD == 2) {
+            const vu2 x = *(const __attribute__((address_space(1))) vu2 *)at;
+            to[0] = x.x, to[1] = x.y;
+        } else {
+            to[0] = *(const __attribute__((address_space(1))) uint32_t *)at;
+        }
+    };
     auto load_tile = [&](int k0) {
+        const char *ka[C::KU], *va[2];
+        bool held = true;
 #pragma unroll
         for (int n = 0; n < C::KU; ++n) {
-            const int pos = k0 + krow + n * (256 / C::PCS);
-            const bool ok = (pos < kb1) & (kpc * 8 < hd) & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
-            const char *at = row_of(Kg, ldk, kid[n], pos);
-            kr[n][0] = *piece(at, ok);
-            kr[n][1] = *piece(at + 16, ok);
+            ka[n] = row_of(Kg, ldk, kid[n], k0 + krow + n * (256 / C::PCS));
+            held = held & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int pos = k0 + (i >> 2) * 16 + 4 * wave + (i & 3);
-            const bool ok = (pos < kb1) & (vd < hd) & (!p.table | ((uint32_t)vid[i >> 2] < (uint32_t)p.n_pages));
-            const auto at = piece(row_of(Vg, ldv, vid[i >> 2], pos), ok);
-            if constexpr (C::VD == 4) {
-                const vu4 x = *at;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) vr[i][e] = x[e];
-            } else if constexpr (C::VD == 2) {
-                const vu2 x = *(const __attribute__((address_space(1))) vu2 *)at;
-                vr[i][0] = x.x, vr[i][1] = x.y;
-            } else {
-                vr[i][0] = *(const __attribute__((address_space(1))) uint32_t *)at;
-            }
+        for (int a = 0; a < 2; ++a) {
+            va[a] = row_of(Vg, ldv, vid[a], k0 + 16 * a + 4 * wave);
+            held = held & (!p.table | ((uint32_t)vid[a] < (uint32_t)p.n_pages));
         }
+        if (hd == HD && k0 + BN <= kb1 && __all(held)) {
+#pragma unroll
+            for (int n = 0; n < C::KU; ++n) kr[n][0] = *(gvu4)(uintptr_t)ka[n], kr[n][1] = *(gvu4)(uintptr_t)(ka[n] + 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) take_v(vr[i], (gvu4)(uintptr_t)(va[i >> 2] + (i & 3) * ldv));
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < C::KU; ++n) {
+            const bool ok = (k0 + krow + n * (256 / C::PCS) < kb1) & (kpc * 8 < hd) & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
+            kr[n][0] = *piece(ka[n], ok);
+            kr[n][1] = *piece(ka[n] + 16, ok);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            take_v(vr[i], piece(va[i >> 2] + (i & 3) * ldv, (k0 + (i >> 2) * 16 + 4 * wave + (i & 3) < kb1) & (vd < hd) &
+                                                                (!p.table | ((uint32_t)vid[i >> 2] < (uint32_t)p.n_pages))));
     };
     char *const Kw = lds + ((krow >> 4) * C::PCS + kpc) * C::KCH + (krow & 15) * 16;
     char *const Vw = lds + 3 * C::KP + (lane >> 4) * C::VD * 1024 + (wave * 16 + l16) * 16;
@@ -806,19 +825,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
         if (k0 <= lim_hi) {
             vf4 s[2] = {vf4{0.0f, 0.0f, 0.0f, 0.0f}, vf4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-            for (int j = 0; j < C::STEPS; ++j)
+            for (int j = 0; j < C::STEPS; ++j) {
+                vu4 k[2][3];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    vu4 k[3];
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int y = 0; y < 3; ++y) k[y] = *(const vu4 *)(Kr + y * C::KP + (b * C::PCS + 4 * j) * C::KCH);
-                    s[b] = mfma_bf16(k[2], qf[0][j], s[b]);
-                    s[b] = mfma_bf16(k[1], qf[1][j], s[b]);
-                    s[b] = mfma_bf16(k[0], qf[2][j], s[b]);
-                    s[b] = mfma_bf16(k[1], qf[0][j], s[b]);
-                    s[b] = mfma_bf16(k[0], qf[1][j], s[b]);
-                    s[b] = mfma_bf16(k[0], qf[0][j], s[b]);
-                }
+                    for (int y = 0; y < 3; ++y) k[b][y] = *(const vu4 *)(Kr + y * C::KP + (b * C::PCS + 4 * j) * C::KCH);
+#pragma unroll
+                for (int x = 0; x < 6; ++x)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) s[b] = mfma_bf16(k[b][SPLIT_A[x]], qf[SPLIT_B[x]][j], s[b]);
+            }
             if (k0 + BN - 1 > lim_lo) {
                 int lim = row.lim - k0 - 4 * g4;
                 asm volatile("" : "+v"(lim));
@@ -858,16 +875,16 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
                     w[0][b * 2 + i / 2] = u[0], w[1][b * 2 + i / 2] = u[1], w[2][b * 2 + i / 2] = u[2];
                 }
 #pragma unroll
-            for (int t = 0; t < C::VT; ++t) {
-                vu4 v[3];
+            for (int t = 0; t < C::VT; t += 2) {
+                vu4 v[2][3];
 #pragma unroll
-                for (int y = 0; y < 3; ++y) v[y] = *(const vu4 *)(Vr + y * C::VP + t * 1024);
-                o[t] = mfma_bf16(v[2], w[0], o[t]);
-                o[t] = mfma_bf16(v[1], w[1], o[t]);
-                o[t] = mfma_bf16(v[0], w[2], o[t]);
-                o[t] = mfma_bf16(v[1], w[0], o[t]);
-                o[t] = mfma_bf16(v[0], w[1], o[t]);
-                o[t] = mfma_bf16(v[0], w[0], o[t]);
+                for (int z = 0; z < 2; ++z)
+#pragma unroll
+                    for (int y = 0; y < 3; ++y) v[z][y] = *(const vu4 *)(Vr + y * C::VP + (t + z) * 1024);
+#pragma unroll
+                for (int x = 0; x < 6; ++x)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) o[t + z] = mfma_bf16(v[z][SPLIT_A[x]], w[SPLIT_B[x]], o[t + z]);
             }
         }
         __syncthreads();
