@@ -352,27 +352,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
     const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
     if (it.part > 0 && kb0 >= kb1) return;
-    const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
-    // this wave's rows: the largest and the smallest last key
-    int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lim_hi = max(lim_hi, __shfl_xor(lim_hi, o, WAVE));
-        lim_lo = min(lim_lo, __shfl_xor(lim_lo, o, WAVE));
-    }
-    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-
-    // queries: B operand, piece 2 j + half of the row
-    vu4 qf[C::STEPS];
-    {
-        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
-#pragma unroll
-        for (int j = 0; j < C::STEPS; ++j) {
-            const int e = (2 * j + half) * C::EP;
-            qf[j] = *piece(Q + e, row.valid && e < hd);
-        }
-    }
-
     // This thread's units: 8 rows x one piece of K or V, rows set * 8 + i (V of 16-bit types:
     // in the order of the weights' registers), in two groups of four neighbours.
     constexpr bool BOTH = C::UPT == 2;  // every thread has a unit of each
@@ -447,6 +426,32 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         }
     };
 
+    if (kb0 < kb1) {
+        load_ids(kb0);
+        load_tile(kb0);
+        load_ids(kb0 + BN);
+    }
+    const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
+    // this wave's rows: the largest and the smallest last key
+    int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lim_hi = max(lim_hi, __shfl_xor(lim_hi, o, WAVE));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, o, WAVE));
+    }
+    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+
+    // queries: B operand, piece 2 j + half of the row
+    vu4 qf[C::STEPS];
+    {
+        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
+#pragma unroll
+        for (int j = 0; j < C::STEPS; ++j) {
+            const int e = (2 * j + half) * C::EP;
+            qf[j] = *piece(Q + e, row.valid && e < hd);
+        }
+    }
+
     const float c = p.scale * LOG2E;
     // The weights' base m follows the maximum only where that is past it by a factor of
     // 2^8: they stay below 2^8, and O is seldom rescaled.
@@ -458,12 +463,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
 
-    if (kb0 < kb1) {
-        load_ids(kb0);
-        load_tile(kb0);
-        load_ids(kb0 + BN);
-        store_tile(0);
-    }
+    if (kb0 < kb1) store_tile(0);
     // The queries are waited for here: in the loop that wait, repeated, would be one for the
     // next tile's rows.
 #pragma unroll
@@ -682,15 +682,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
     const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
     if (it.part > 0 && kb0 >= kb1) return;
-    const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 16 + l16, group, g);
-    int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
-#pragma unroll
-    for (int x = 8; x > 0; x >>= 1) {
-        lim_hi = max(lim_hi, __shfl_xor(lim_hi, x, WAVE));
-        lim_lo = min(lim_lo, __shfl_xor(lim_lo, x, WAVE));
-    }
-    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-
     // K: rows tid / PCS (and 256 / PCS on), dimensions 8 (tid % PCS); V: dimensions VD (tid % 64) of
     // the wave's eight keys 4 w + 0..3, 16 + 4 w + 0..3
     const int kpc = tid % C::PCS, krow = tid / C::PCS, vd = lane * C::VD;
@@ -793,6 +784,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
         load_tile(kb0);
         load_ids(kb0 + BN);
     }
+    const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 16 + l16, group, g);
+    int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) {
+        lim_hi = max(lim_hi, __shfl_xor(lim_hi, x, WAVE));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, x, WAVE));
+    }
+    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
     {
         const float *Q = (const float *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
 #pragma unroll
@@ -977,28 +976,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend - from);
     const int part = plan.part0 + it.part, kb0 = min(from + it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
     if (it.part > 0 && kb0 >= kb1) return;
-    int lim[NQ], lim_hi = -1, lim_lo = INT32_MAX;
-    vu4 qf[NQ][C::STEPS];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const Row row = row_at<PREFIX>(p, q, tile * BM + n * 16 + l16, group, g);
-        lim[n] = row.lim;
-        lim_hi = max(lim_hi, lim[n]);
-        if (row.valid) lim_lo = min(lim_lo, lim[n]);
-        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
-#pragma unroll
-        for (int j = 0; j < C::STEPS; ++j) {
-            const int e = (4 * j + g4) * C::EP;
-            qf[n][j] = *piece(Q + e, row.valid && e < hd);
-        }
-    }
-#pragma unroll
-    for (int x = 8; x > 0; x >>= 1) {
-        lim_hi = max(lim_hi, __shfl_xor(lim_hi, x, WAVE));
-        lim_lo = min(lim_lo, __shfl_xor(lim_lo, x, WAVE));
-    }
-    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-
     const char *const Kg = (const char *)((const T *)p.k + (int64_t)g * hd), *const Vg = (const char *)((const T *)p.v + (int64_t)g * hd);
     const uint32_t ldk = (uint32_t)p.ldk * sizeof(T), ldv = (uint32_t)p.ldv * sizeof(T);
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
@@ -1075,6 +1052,38 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
             }
         }
     };
+
+    constexpr int STRIDE = 4 * C::KS;
+    const int first = kb0 + wave * C::KS;
+    Step now, next;
+    Ids ids;
+    if (first < kb1) {
+        load_ids(ids, first);
+        const Ids held = ids;
+        load_ids(ids, first + STRIDE);
+        load(now, held, first);
+    }
+    int lim[NQ], lim_hi = -1, lim_lo = INT32_MAX;
+    vu4 qf[NQ][C::STEPS];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const Row row = row_at<PREFIX>(p, q, tile * BM + n * 16 + l16, group, g);
+        lim[n] = row.lim;
+        lim_hi = max(lim_hi, lim[n]);
+        if (row.valid) lim_lo = min(lim_lo, lim[n]);
+        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
+#pragma unroll
+        for (int j = 0; j < C::STEPS; ++j) {
+            const int e = (4 * j + g4) * C::EP;
+            qf[n][j] = *piece(Q + e, row.valid && e < hd);
+        }
+    }
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) {
+        lim_hi = max(lim_hi, __shfl_xor(lim_hi, x, WAVE));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, x, WAVE));
+    }
+    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
 
     const float c = p.scale * LOG2E, slack = 8.0f / c;  // (as in the tiles)
     float m[NQ], l[NQ];
@@ -1169,28 +1178,20 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     };
 
     // The next step in flight during a step's products, the page ids of the one after it ahead
-    // of that (loads return in order: a wait for an id must not be one for rows).  One copy of
-    // the code, for the instruction cache: HBM leaves time for the moves.
-    constexpr int STRIDE = 4 * C::KS;
-    const int first = kb0 + wave * C::KS, stop = min(kb1, lim_hi + 1);
-    if (first < stop) {
-        Step now, next;
-        Ids ids;
-        load_ids(ids, first);
+    // of that (loads return in order: a wait for an id must not be one for rows).
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[n][j]));  // (waited for here, as in the tiles)
-        for (int k0 = first - STRIDE;; k0 += STRIDE) {
-            if (k0 + STRIDE < stop) {
-                const Ids held = ids;
-                load_ids(ids, k0 + 2 * STRIDE);
-                load(next, held, k0 + STRIDE);
-            }
-            if (k0 >= first) compute(now, k0);
-            if (k0 + STRIDE >= stop) break;
-            now = next;
+        for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[n][j]));  // (waited for here, as in the tiles)
+    const int stop = min(kb1, lim_hi + 1);
+    for (int k0 = first; k0 < stop; k0 += STRIDE) {
+        if (k0 + STRIDE < stop) {
+            const Ids held = ids;
+            load_ids(ids, k0 + 2 * STRIDE);
+            load(next, held, k0 + STRIDE);
         }
+        compute(now, k0);
+        now = next;
     }
 
     // the four waves' results: each to the common maximum, then summed
@@ -1344,7 +1345,7 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     const int large = p.dtype == GAJE_DTYPE_F32 ? 64 : 128;
     t.bm = avg <= small || key0 > 0 ? small : large;  // (the tiles begin with key 0)
     t.key0 = (int32_t)key0;
-    t.least = t.bm >= 64 ? 256 : 128;
+    t.least = prefix ? 128 : t.bm >= 64 ? 512 : 128;
     t.blocks = 9;
     const int target = 1 << t.blocks;
     // ragged sequences end in a tile that is not full
