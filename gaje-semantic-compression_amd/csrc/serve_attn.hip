@@ -20,6 +20,8 @@ namespace gaje {
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
+// a factor of 2^8 between weights, in scores (finite for every scale)
+__device__ __forceinline__ float slack_of(float c) { return fminf(8.0f / c, 1e30f); }
 
 typedef float vf16 __attribute__((ext_vector_type(16)));
 typedef _Float16 vh8 __attribute__((ext_vector_type(8)));
@@ -31,6 +33,22 @@ __device__ const vu4 zero_piece = {0, 0, 0, 0};
 typedef const __attribute__((address_space(1))) vu4 *gvu4;
 typedef const __attribute__((address_space(1))) char *gchar;
 __device__ __forceinline__ gvu4 piece(const void *p, bool ok) { return ok ? (gvu4)(uintptr_t)p : (gvu4)(uintptr_t)&zero_piece; }
+
+// 16 x 16 and 32 x 32 products of 16-bit operands, eight of a lane's at a time.
+template <typename T>
+__device__ __forceinline__ vf4 mfma16(vu4 a, vu4 b, vf4 c) {
+    if constexpr (std::is_same<T, _Float16>::value)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vh8, a), __builtin_bit_cast(vh8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, b), c, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ vf16 mfma32(vu4 a, vu4 b, vf16 c) {
+    if constexpr (std::is_same<T, _Float16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, a), __builtin_bit_cast(vh8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, b), c, 0, 0, 0);
+}
 
 // Prefix sums (and running maxima of values >= 0) over the wave, by cross-lane moves
 // within the VALU.
@@ -162,21 +180,19 @@ __device__ __forceinline__ int seq_of_row(const ServeAttnParams &p, int t) {
 // leave their registers.  K and V are staged in LDS in operand order (V transposed on
 // the way, 8 keys x 8 dimensions per thread with v_perm), so that every operand is one
 // conflict-free 16-byte read; two buffers, one barrier per tile, the next tile's global
-// loads in flight during a tile's products.  f32 runs the f32 matrix instructions (no
-// transposition: one key per half-wave and step).
+// loads in flight during a tile's products.
+// Bound by the matrix and vector units in turn (46% and 48% of the cycles at 8190 rows, 32
+// heads of 128: one exponential per 2 * 128 products), which two waves of a SIMD seldom overlap.
 template <typename T, int HD>
 struct TileCfg {
-    static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int BN = F32 ? (HD == 64 ? 64 : 32) : 8192 / HD;  // keys per tile
-    static constexpr int EP = 16 / sizeof(T);                          // elements per 16-byte piece
-    static constexpr int PCS = HD / EP;                                // pieces per row
-    static constexpr int UNITS = BN / 8 * PCS;                         // of 8 rows x one piece, K or V
-    static constexpr int UPT = 2 * UNITS / 256;                        // units per thread
-    static constexpr int NT = HD / 32;                                 // 32-dimension blocks of O^T
-    static constexpr int KROW = 32 * 16 + 16;                          // bytes of 32 keys' pieces in LDS, 4 banks on
-    static constexpr int KT = BN / 32 * PCS * KROW, VT = BN * HD * (int)sizeof(T);
+    static_assert(sizeof(T) == 2, "f32 has tiles of its own");
+    static constexpr int BN = 8192 / HD;               // keys per tile
+    static constexpr int PCS = HD / 8;                 // 16-byte pieces per row
+    static constexpr int NT = HD / 32;                 // 32-dimension blocks of O^T
+    static constexpr int KROW = 32 * 16 + 16;          // bytes of 32 keys' pieces in LDS, 4 banks on
+    static constexpr int KT = BN / 32 * PCS * KROW, VT = BN * HD * 2;
     static constexpr int LDS = 2 * (KT + VT);
-    static constexpr int STEPS = HD / (F32 ? 8 : 16);                  // of the scores' operands
+    static constexpr int STEPS = HD / 16;              // of the scores' operands
 };
 
 struct TilePlan {
@@ -336,92 +352,74 @@ __device__ __forceinline__ void store_row(const ServeAttnParams &p, int64_t t, i
 }
 
 template <typename T, int HD, bool PREFIX>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(ServeAttnParams p, TilePlan plan) {
+__device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
     using C = TileCfg<T, HD>;
     constexpr int BM = 128, BN = C::BN, NB = BN / 32;
-    extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, l32 = lane & 31;
-    const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
+    const int group = p.n_head / p.n_head_kv, g = block % p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX, true>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
-    if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    if (!find_item<PREFIX, true>(p, plan, block / p.n_head_kv, group, it)) return;
+    if (!PREFIX && block == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
     const int tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
     const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
     if (it.part > 0 && kb0 >= kb1) return;
-    // This thread's units: 8 rows x one piece of K or V, rows set * 8 + i (V of 16-bit types:
-    // in the order of the weights' registers), in two groups of four neighbours.
-    constexpr bool BOTH = C::UPT == 2;  // every thread has a unit of each
-    const int unit = BOTH ? tid : tid & 127, pc = unit % C::PCS, set = unit / C::PCS;
-    const bool in = pc * C::EP < hd;
-    auto is_v = [&](int n) { return BOTH ? n == 1 : wave >= 2; };
-    auto group_of = [&](bool v, int a) { return C::F32 || !v ? set * 8 + 4 * a : (set >> 1) * 16 + (set & 1) * 4 + 8 * a; };
-    vu4 rg[C::UPT][8];
-    int ids[C::UPT][2];
+    // This thread's unit: 8 rows x one piece, of K for the first two waves, of V for the others;
+    // rows set * 8 + i, or V's in the order of the weights' registers, in two groups of four.
+    const bool is_v = wave >= 2;
+    const int unit = tid & 127, pc = unit % C::PCS, set = unit / C::PCS;
+    int rows_at[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) rows_at[a] = is_v ? (set >> 1) * 16 + (set & 1) * 4 + 8 * a : set * 8 + 4 * a;
+    const char *const base = (const char *)((const T *)(is_v ? p.v : p.k) + (int64_t)g * hd) + pc * 16;
+    const uint32_t ld = (uint32_t)(is_v ? p.ldv : p.ldk) * sizeof(T);
+    vu4 rg[8];
+    int ids[2];
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
     const int page_mask = (1 << p.page_shift) - 1;
     auto load_ids = [&](int k0) {
         if (!p.table) return;
 #pragma unroll
-        for (int n = 0; n < C::UPT; ++n)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) ids[n][a] = pages[min(k0 + group_of(is_v(n), a), kb1 - 1) >> p.page_shift];
+        for (int a = 0; a < 2; ++a) ids[a] = pages[min(k0 + rows_at[a], kb1 - 1) >> p.page_shift];
     };
     auto load_tile = [&](int k0) {
+        const char *at[2];
+        bool held[2] = {true, true};
 #pragma unroll
-        for (int n = 0; n < C::UPT; ++n) {
-            const bool v = is_v(n);
-            const char *base = (const char *)((v ? (const T *)p.v : (const T *)p.k) + (int64_t)g * hd);
-            const uint32_t ld = (uint32_t)(v ? p.ldv : p.ldk) * sizeof(T);
-            const char *at[2];
-            bool held[2] = {true, true};
+        for (int a = 0; a < 2; ++a) {
             if (p.table) {
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    held[a] = (uint32_t)ids[n][a] < (uint32_t)p.n_pages;
-                    const uint32_t in_page = (uint32_t)((k0 + group_of(v, a)) & page_mask) * ld + pc * 16;
-                    at[a] = base + in_page + (uint64_t)(uint32_t)ids[n][a] * (ld << p.page_shift);
-                }
+                held[a] = (uint32_t)ids[a] < (uint32_t)p.n_pages;
+                at[a] = base + (uint32_t)((k0 + rows_at[a]) & page_mask) * ld + (uint64_t)(uint32_t)ids[a] * (ld << p.page_shift);
             } else {
-                const char *tile0 = base + (int64_t)(q.row0 + k0) * ld;
-#pragma unroll
-                for (int a = 0; a < 2; ++a) at[a] = tile0 + (uint32_t)group_of(v, a) * ld + pc * 16;
+                at[a] = base + (int64_t)(q.row0 + k0) * ld + (uint32_t)rows_at[a] * ld;
             }
-            if (k0 + BN <= kb1 && hd == HD && __all(held[0] & held[1])) {
+        }
+        if (k0 + BN <= kb1 && hd == HD && __all(held[0] & held[1])) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) rg[n][i] = *(gvu4)(uintptr_t)(at[i >> 2] + (i & 3) * ld);
-            } else {
+            for (int i = 0; i < 8; ++i) rg[i] = *(gvu4)(uintptr_t)(at[i >> 2] + (i & 3) * ld);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool ok = in & (k0 + group_of(v, i >> 2) + (i & 3) < kb1) & held[i >> 2];
-                    rg[n][i] = *piece(at[i >> 2] + (i & 3) * ld, ok);
-                }
-            }
+            for (int i = 0; i < 8; ++i)
+                rg[i] = *piece(at[i >> 2] + (i & 3) * ld, (pc * 8 < hd) & (k0 + rows_at[i >> 2] + (i & 3) < kb1) & held[i >> 2]);
         }
     };
     char *const Kw = lds + ((set >> 2) * C::PCS + pc) * C::KROW + (set & 3) * 128;
-    char *const Vw = lds + 2 * C::KT + (C::F32 ? (set * 8 * C::PCS + pc) * 16 : (set >> 1) * C::NT * 1024 + (set & 1) * 512 + pc * 16);
+    char *const Vw = lds + 2 * C::KT + (set >> 1) * C::NT * 1024 + (set & 1) * 512 + pc * 16;
     auto store_tile = [&](int buf) {
+        if (!is_v) {
 #pragma unroll
-        for (int n = 0; n < C::UPT; ++n) {
-            if (!is_v(n)) {
+            for (int i = 0; i < 8; ++i) *(vu4 *)(Kw + buf * C::KT + i * 16) = rg[i];
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) *(vu4 *)(Kw + buf * C::KT + i * 16) = rg[n][i];
-            } else if constexpr (C::F32) {
+            for (int e = 0; e < 8; ++e) {
+                vu4 w;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) *(vu4 *)(Vw + buf * C::VT + i * C::PCS * 16) = rg[n][i];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    vu4 w;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        w[k] = __builtin_amdgcn_perm(rg[n][2 * k + 1][e >> 1], rg[n][2 * k][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-                    *(vu4 *)(Vw + buf * C::VT + (e % C::NT) * 1024 + (e / C::NT) * C::PCS * 16) = w;
-                }
+                for (int k = 0; k < 4; ++k)
+                    w[k] = __builtin_amdgcn_perm(rg[2 * k + 1][e >> 1], rg[2 * k][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                *(vu4 *)(Vw + buf * C::VT + (e % C::NT) * 1024 + (e / C::NT) * C::PCS * 16) = w;
             }
         }
     };
@@ -447,7 +445,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
         const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
 #pragma unroll
         for (int j = 0; j < C::STEPS; ++j) {
-            const int e = (2 * j + half) * C::EP;
+            const int e = (2 * j + half) * 8;
             qf[j] = *piece(Q + e, row.valid && e < hd);
         }
     }
@@ -455,7 +453,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     const float c = p.scale * LOG2E;
     // The weights' base m follows the maximum only where that is past it by a factor of
     // 2^8: they stay below 2^8, and O is seldom rescaled.
-    const float slack = 8.0f / c;
+    const float slack = slack_of(c);
     float m = -INFINITY, l = 0.0f;
     vf16 o[C::NT];
 #pragma unroll
@@ -470,7 +468,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
     for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[j]));
     __syncthreads();
     const char *const Kr = lds + half * C::KROW + l32 * 16;
-    const char *const Vr = lds + 2 * C::KT + (C::F32 ? half * 4 * HD * 4 + l32 * (C::NT == 2 ? 8 : 16) : lane * 16);
+    const char *const Vr = lds + 2 * C::KT + lane * 16;
     int buf = 0;
     for (int k0 = kb0; k0 < kb1; k0 += BN, buf ^= 1) {
         const bool more = k0 + BN < kb1;
@@ -491,15 +489,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const vu4 kf = *(const vu4 *)(Kl + (b * C::PCS + 2 * j) * C::KROW);
-                    if constexpr (C::F32) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[i]), __uint_as_float(qf[j][i]), s[b], 0, 0, 0);
-                    } else if constexpr (std::is_same<T, _Float16>::value) {
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, kf), __builtin_bit_cast(vh8, qf[j]), s[b], 0, 0, 0);
-                    } else {
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, kf), __builtin_bit_cast(vb8, qf[j]), s[b], 0, 0, 0);
-                    }
+                    s[b] = mfma32<T>(kf, qf[j], s[b]);
                 }
             if (k0 + BN - 1 > lim_lo) {
                 int lim = row.lim - k0 - 4 * half;
@@ -538,39 +528,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
             l += sum;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if constexpr (C::F32) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const char *vr = Vl + (b * 32 + 8 * (i >> 2) + (i & 3)) * HD * 4;
-                        float vv[C::NT];
-                        if constexpr (C::NT == 2) {
-                            const float2 a = *(const float2 *)vr;
-                            vv[0] = a.x, vv[1] = a.y;
-                        } else {
+                for (int st = 0; st < 2; ++st) {
+                    // (rounded to the type, to nearest even: as far off as the result's own rounding)
+                    union { T e[8]; vu4 u; } w;
 #pragma unroll
-                            for (int t = 0; t < C::NT; t += 4) {
-                                const float4 a = *(const float4 *)(vr + t * 128);
-                                vv[t] = a.x, vv[t + 1] = a.y, vv[t + 2] = a.z, vv[t + 3] = a.w;
-                            }
-                        }
+                    for (int i = 0; i < 8; ++i) w.e[i] = (T)s[b][8 * st + i];
 #pragma unroll
-                        for (int t = 0; t < C::NT; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv[t], s[b][i], o[t], 0, 0, 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        T w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = (T)s[b][8 * st + i];
-#pragma unroll
-                        for (int t = 0; t < C::NT; ++t) {
-                            const vu4 vf = *(const vu4 *)(Vl + ((b * 2 + st) * C::NT + t) * 1024);
-                            if constexpr (std::is_same<T, _Float16>::value)
-                                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh8, vf), __builtin_bit_cast(vh8, w), o[t], 0, 0, 0);
-                            else
-                                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vb8, vf), __builtin_bit_cast(vb8, w), o[t], 0, 0, 0);
-                        }
-                    }
+                    for (int t = 0; t < C::NT; ++t)
+                        o[t] = mfma32<T>(*(const vu4 *)(Vl + ((b * 2 + st) * C::NT + t) * 1024), w.u, o[t]);
                 }
             }
         }
@@ -599,21 +565,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_tile_kernel(Serve
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int r = 8 * (i >> 2) + 4 * half + (i & 3);
-            // dimensions of row r of the blocks: NT (f32 of 256: twice 4) neighbours
-            constexpr int RUN = C::F32 && C::NT == 8 ? 4 : C::NT;
+            // row r of the blocks: NT neighbouring dimensions
+            const int d = (r % C::PCS) * 8 + (r / C::PCS) * C::NT;
+            if (d >= hd) continue;
+            if (whole) {
+                T e[C::NT];
 #pragma unroll
-            for (int t0 = 0; t0 < C::NT; t0 += RUN) {
-                const int d = C::F32 ? t0 * 32 + r * RUN : (r % C::PCS) * 8 + (r / C::PCS) * C::NT;
-                if (d >= hd) continue;
-                if (whole) {
-                    T e[RUN];
+                for (int t = 0; t < C::NT; ++t) e[t] = (T)(o[t][i] * inv);
+                __builtin_memcpy(__builtin_assume_aligned(out + d, sizeof e), e, sizeof e);
+            } else {
 #pragma unroll
-                    for (int t = 0; t < RUN; ++t) e[t] = (T)(o[t0 + t][i] * inv);
-                    __builtin_memcpy(__builtin_assume_aligned(out + d, RUN * sizeof(T) > 16 ? 16 : RUN * sizeof(T)), e, sizeof e);
-                } else {
-#pragma unroll
-                    for (int t = 0; t < RUN; ++t) po[d + t] = o[t0 + t][i];
-                }
+                for (int t = 0; t < C::NT; ++t) po[d + t] = o[t][i];
             }
         }
         if (!whole && half == 0) p.part_ml[at] = make_float2(m, l);
@@ -661,21 +623,16 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
 }
 // the products, the smallest first
 constexpr int SPLIT_A[6] = {2, 1, 0, 1, 0, 0}, SPLIT_B[6] = {0, 1, 2, 0, 1, 0};
-__device__ __forceinline__ vf4 mfma_bf16(vu4 a, vu4 b, vf4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, b), c, 0, 0, 0);
-}
-
 template <int HD, bool PREFIX>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(ServeAttnParams p, TilePlan plan) {
+__device__ __forceinline__ void attend_split(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
     using C = SplitCfg<HD>;
     constexpr int BM = C::BM, BN = C::BN;
-    extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g4 = lane >> 4;
-    const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
+    const int group = p.n_head / p.n_head_kv, g = block % p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX, true>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
-    if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    if (!find_item<PREFIX, true>(p, plan, block / p.n_head_kv, group, it)) return;
+    if (!PREFIX && block == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
     const int tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
@@ -808,7 +765,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
             }
         }
     }
-    const float c = p.scale * LOG2E, slack = 8.0f / c;  // (as in the tiles)
+    const float c = p.scale * LOG2E, slack = slack_of(c);  // (as in the tiles)
     float m = -INFINITY, l = 0.0f;
     vf4 o[C::VT];
 #pragma unroll
@@ -833,7 +790,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
 #pragma unroll
                 for (int x = 0; x < 6; ++x)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) s[b] = mfma_bf16(k[b][SPLIT_A[x]], qf[SPLIT_B[x]][j], s[b]);
+                    for (int b = 0; b < 2; ++b) s[b] = mfma16<__bf16>(k[b][SPLIT_A[x]], qf[SPLIT_B[x]][j], s[b]);
             }
             if (k0 + BN - 1 > lim_lo) {
                 int lim = row.lim - k0 - 4 * g4;
@@ -883,7 +840,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
 #pragma unroll
                 for (int x = 0; x < 6; ++x)
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) o[t + z] = mfma_bf16(v[z][SPLIT_A[x]], w[SPLIT_B[x]], o[t + z]);
+                    for (int z = 0; z < 2; ++z) o[t + z] = mfma16<__bf16>(v[z][SPLIT_A[x]], w[SPLIT_B[x]], o[t + z]);
             }
         }
         __syncthreads();
@@ -933,7 +890,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_split_kernel(Serv
 }
 
 // ---- few rows ----
-// A workgroup takes up to 16 NQ query rows of one K/V head (a decoded token's query heads,
+// A workgroup takes up to 16 query rows of one K/V head (a decoded token's query heads,
 // a few drafted tokens), and its four waves take turns at the keys, KS each, every wave
 // with a softmax of its own until they are joined at the end.  Nothing is shared while the
 // keys stream by, so K and V go from memory to registers (two steps of them in flight)
@@ -954,22 +911,29 @@ struct FewCfg {
     static constexpr int VK = 4 * KB;                   // keys of a lane
     static constexpr int VB = VW * (int)sizeof(T);      // bytes of a lane's row of V
     static constexpr int VP = (VB + 15) / 16;           // pieces of it
-    static constexpr int NQ2 = HD == 256 ? 1 : 2;       // blocks of rows where there are more than 16
 };
 
-template <typename T, int HD, int NQ, bool PREFIX>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeAttnParams p, TilePlan plan) {
+template <int HD>
+struct FewLds {
+    float joined[4][16][HD], ms[4][16], ls[4][16];
+    int odd[16];
+};
+
+template <typename T, int HD, bool PREFIX>
+__device__ __forceinline__ void attend_few(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
     using C = FewCfg<T, HD>;
-    constexpr int BM = 16 * NQ;
-    __shared__ __align__(16) float joined[4][BM][HD];
-    __shared__ float ms[4][BM], ls[4][BM];
-    __shared__ int odd[BM];
+    constexpr int BM = 16;
+    FewLds<HD> &sh = *(FewLds<HD> *)lds;
+    auto &joined = sh.joined;
+    auto &ms = sh.ms;
+    auto &ls = sh.ls;
+    auto &odd = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g4 = lane >> 4;
-    const int group = p.n_head / p.n_head_kv, g = blockIdx.x % p.n_head_kv, hd = p.head_dim;
+    const int group = p.n_head / p.n_head_kv, g = block % p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX, false>(p, plan, blockIdx.x / p.n_head_kv, group, it)) return;
-    if (!PREFIX && blockIdx.x == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    if (!find_item<PREFIX, false>(p, plan, block / p.n_head_kv, group, it)) return;
+    if (!PREFIX && block == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
     const Seq q = it.q;
     const int tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group), key0 = min(plan.key0, kend), from = key0 & ~31;
@@ -1063,19 +1027,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
         load_ids(ids, first + STRIDE);
         load(now, held, first);
     }
-    int lim[NQ], lim_hi = -1, lim_lo = INT32_MAX;
-    vu4 qf[NQ][C::STEPS];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const Row row = row_at<PREFIX>(p, q, tile * BM + n * 16 + l16, group, g);
-        lim[n] = row.lim;
-        lim_hi = max(lim_hi, lim[n]);
-        if (row.valid) lim_lo = min(lim_lo, lim[n]);
+    int lim, lim_hi, lim_lo;
+    vu4 qf[C::STEPS];
+    {
+        const Row row = row_at<PREFIX>(p, q, tile * BM + l16, group, g);
+        lim = lim_hi = row.lim;
+        lim_lo = row.valid ? lim : INT32_MAX;
         const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
 #pragma unroll
         for (int j = 0; j < C::STEPS; ++j) {
             const int e = (4 * j + g4) * C::EP;
-            qf[n][j] = *piece(Q + e, row.valid && e < hd);
+            qf[j] = *piece(Q + e, row.valid && e < hd);
         }
     }
 #pragma unroll
@@ -1085,94 +1047,75 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     }
     lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
 
-    const float c = p.scale * LOG2E, slack = 8.0f / c;  // (as in the tiles)
-    float m[NQ], l[NQ];
-    vf4 o[NQ][C::VW];
+    const float c = p.scale * LOG2E, slack = slack_of(c);  // (as in the tiles)
+    float m = -INFINITY, l = 0.0f;
+    vf4 o[C::VW];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        m[n] = -INFINITY, l[n] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < C::VW; ++t) o[n][t] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int t = 0; t < C::VW; ++t) o[t] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
     auto compute = [&](const Step &x, int k0) {
-        vf4 s[NQ][C::KB];
+        vf4 s[C::KB];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int b = 0; b < C::KB; ++b) {
+            s[b] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int b = 0; b < C::KB; ++b) {
-                s[n][b] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < C::STEPS; ++j) {
+                if constexpr (C::F32) {
 #pragma unroll
-                for (int j = 0; j < C::STEPS; ++j) {
-                    if constexpr (C::F32) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[b][j][i]), __uint_as_float(qf[n][j][i]), s[n][b], 0, 0, 0);
-                    } else if constexpr (std::is_same<T, _Float16>::value) {
-                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vh8, x.k[b][j]), __builtin_bit_cast(vh8, qf[n][j]), s[n][b], 0, 0, 0);
-                    } else {
-                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, x.k[b][j]), __builtin_bit_cast(vb8, qf[n][j]), s[n][b], 0, 0, 0);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[b][j][i]), __uint_as_float(qf[j][i]), s[b], 0, 0, 0);
+                } else {
+                    s[b] = mfma16<T>(x.k[b][j], qf[j], s[b]);
                 }
             }
-        T w[NQ][8];
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            if (k0 < key0 || k0 + C::KS - 1 > lim_lo) {
-#pragma unroll
-                for (int b = 0; b < C::KB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int pos = k0 + b * 16 + 4 * g4 + i;
-                        if (pos > lim[n] || pos < key0) s[n][b][i] = -INFINITY;
-                    }
-            }
-            float mt = s[n][0][0];
-#pragma unroll
-            for (int b = 0; b < C::KB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[n][b][i]);
-            mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-            if (__any(mt > m[n] + slack)) {
-                mt = fmaxf(mt, m[n]);
-                const float shrink = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mt) * c);
-                l[n] *= shrink;
-#pragma unroll
-                for (int t = 0; t < C::VW; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[n][t][i] *= shrink;
-                m[n] = mt;
-            }
-            const float base = m[n] == -INFINITY ? 0.0f : m[n] * c;
+        }
+        if (k0 < key0 || k0 + C::KS - 1 > lim_lo) {
 #pragma unroll
             for (int b = 0; b < C::KB; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[n][b][i] = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], c, -base));
-                    l[n] += s[n][b][i];
-                    w[n][4 * b + i] = (T)s[n][b][i];
+                    const int pos = k0 + b * 16 + 4 * g4 + i;
+                    if (pos > lim || pos < key0) s[b][i] = -INFINITY;
                 }
         }
+        float mt = s[0][0];
+#pragma unroll
+        for (int b = 0; b < C::KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[b][i]);
+        mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+        if (__any(mt > m + slack)) {
+            mt = fmaxf(mt, m);
+            const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mt) * c);
+            l *= shrink;
+#pragma unroll
+            for (int t = 0; t < C::VW; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[t][i] *= shrink;
+            m = mt;
+        }
+        const float base = m == -INFINITY ? 0.0f : m * c;
+        union { T e[8]; vu4 u; } w;
+#pragma unroll
+        for (int b = 0; b < C::KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -base));
+                l += s[b][i];
+                if constexpr (!C::F32) w.e[4 * b + i] = (T)s[b][i];
+            }
 #pragma unroll
         for (int t = 0; t < C::VW; ++t) {
             if constexpr (C::F32) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n)
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[i][t >> 2][t & 3]), s[n][0][i], o[n][t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[i][t >> 2][t & 3]), s[0][i], o[t], 0, 0, 0);
             } else {
                 vu4 a;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     a[k] = __builtin_amdgcn_perm(x.v[2 * k + 1][t >> 3][(t & 7) >> 1], x.v[2 * k][t >> 3][(t & 7) >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    if constexpr (std::is_same<T, _Float16>::value)
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vh8, a), __builtin_bit_cast(vh8, w[n]), o[n][t], 0, 0, 0);
-                    else
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vb8, a), __builtin_bit_cast(vb8, w[n]), o[n][t], 0, 0, 0);
-                }
+                o[t] = mfma16<T>(a, w.u, o[t]);
             }
         }
     };
@@ -1180,9 +1123,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     // The next step in flight during a step's products, the page ids of the one after it ahead
     // of that (loads return in order: a wait for an id must not be one for rows).
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[n][j]));  // (waited for here, as in the tiles)
+    for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[j]));  // (waited for here, as in the tiles)
     const int stop = min(kb1, lim_hi + 1);
     for (int k0 = first; k0 < stop; k0 += STRIDE) {
         if (k0 + STRIDE < stop) {
@@ -1195,25 +1136,21 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
     }
 
     // the four waves' results: each to the common maximum, then summed
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        l[n] += __shfl_xor(l[n], 16, WAVE);
-        l[n] += __shfl_xor(l[n], 32, WAVE);
-        if (g4 == 0) ms[wave][n * 16 + l16] = m[n], ls[wave][n * 16 + l16] = l[n];
-    }
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+    if (g4 == 0) ms[wave][l16] = m, ls[wave][l16] = l;
     if (tid < BM) odd[tid] = 0;
     __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
+    {
         float mt = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ms[w][n * 16 + l16]);
+        for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ms[w][l16]);
         const float base = mt == -INFINITY ? 0.0f : mt * c;
-        const float shrink = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m[n], c, -base));
+        const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m, c, -base));
 #pragma unroll
         for (int t = 0; t < C::VW; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) joined[wave][n * 16 + l16][(4 * g4 + i) * C::VW + t] = m[n] == -INFINITY ? 0.0f : o[n][t][i] * shrink;
+            for (int i = 0; i < 4; ++i) joined[wave][l16][(4 * g4 + i) * C::VW + t] = m == -INFINITY ? 0.0f : o[t][i] * shrink;
     }
     __syncthreads();
     // 256 / BM threads per row
@@ -1270,6 +1207,36 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_few_kernel(ServeA
         attend_row<T>(p, qs, w.t, w.head, max(kb0, key0), min(kb1, w.lim + 1), mr, lr, orow);
         store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
     }
+}
+
+// ---- launches ----
+// A plan's rows: 16 per workgroup by the few-row form, 64 (f32) or 128 by tiles.
+enum RowForm { ROWS_FEW, ROWS_TILE };
+template <typename T, int HD, RowForm FORM, bool PREFIX>
+__device__ __forceinline__ void attend(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
+    if constexpr (FORM == ROWS_FEW) attend_few<T, HD, PREFIX>(p, plan, block, lds);
+    else if constexpr (sizeof(T) == 4) attend_split<HD, PREFIX>(p, plan, block, lds);
+    else attend_tile<T, HD, PREFIX>(p, plan, block, lds);
+}
+template <typename T, int HD, RowForm FORM>
+constexpr size_t lds_of() {
+    if constexpr (FORM == ROWS_FEW) return sizeof(FewLds<HD>);
+    else if constexpr (sizeof(T) == 4) return SplitCfg<HD>::LDS;
+    else return TileCfg<T, HD>::LDS;
+}
+
+template <typename T, int HD, RowForm FORM>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_kernel(ServeAttnParams p, TilePlan keys) {
+    extern __shared__ __align__(16) char lds[];
+    attend<T, HD, FORM, false>(p, keys, blockIdx.x, lds);
+}
+// The shared prefix by the first workgroups, the sequences' own keys by the others.
+template <typename T, int HD, RowForm FORM>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_prefix_kernel(ServeAttnParams p, TilePlan prefix, TilePlan keys) {
+    extern __shared__ __align__(16) char lds[];
+    const int blocks = (int)prefix.items * p.n_head_kv;
+    if ((int)blockIdx.x < blocks) attend<T, HD, FORM, true>(p, prefix, blockIdx.x, lds);
+    else attend<T, HD, ROWS_FEW, false>(p, keys, blockIdx.x - blocks, lds);
 }
 
 // ---- joining parts ----
@@ -1341,12 +1308,18 @@ struct AttnPlan {
 TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t most, int64_t key0, bool prefix) {
     TilePlan t{};
     const int64_t avg = rows / std::max<int64_t>(seqs, 1);
-    const int small = avg <= 16 || p.head_dim > 128 ? 16 : 32;
-    const int large = p.dtype == GAJE_DTYPE_F32 ? 64 : 128;
-    t.bm = avg <= small || key0 > 0 ? small : large;  // (the tiles begin with key 0)
+    // Up to 16 rows of a sequence: the few-row form, which the tiles pass soon after (32
+    // sequences of 500 to 2000 keys, 12 heads of 128: 30 rows bf16 22.4 against 20.2 us, f32
+    // 38.7 against 37.3).  After a prefix it is always that: the tiles begin with key 0.
+    t.bm = avg <= 16 || key0 > 0 ? 16 : p.dtype == GAJE_DTYPE_F32 ? 64 : 128;
     t.key0 = (int32_t)key0;
-    t.least = prefix ? 128 : t.bm >= 64 ? 512 : 128;
-    t.blocks = 9;
+    // Workgroups wanted: two for each of 256 CUs; over a prefix one, where every part costs
+    // partial results of all rows (64 sequences over 16000 keys: 29.1 against 38.2 us).
+    t.blocks = prefix ? 8 : 9;
+    // Parts of a prompt's own keys pay from 512 keys on (f32 prompts of up to 1500 tokens 67.6
+    // against 75.1 us with 256, one f16 prompt of 1500 34.1 against 42.6), of a cache's from 256 (5
+    // drafted tokens, f32, 37.3 against 49.4), a few rows' and a prefix's from 128.
+    t.least = prefix || t.bm == 16 ? 128 : p.table ? 256 : 512;
     const int target = 1 << t.blocks;
     // ragged sequences end in a tile that is not full
     const int64_t tiles = prefix || p.prefix_table ? seqs * ((rows / seqs + t.bm - 1) / t.bm) : rows / t.bm + std::min(seqs, p.T);
@@ -1383,52 +1356,47 @@ AttnPlan make_plan(const ServeAttnParams &p) {
     return a;
 }
 
-template <typename T, int HD, bool PREFIX>
-int launch_tiles(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
-    const int64_t blocks = plan.items * p.n_head_kv;
+int set_lds(const void *kernel, size_t lds, std::atomic<bool> *set) {
+    int dev = 0;
+    GAJE_HIP_CHECK(hipGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && set[dev].load()) return GAJE_OK;
+    GAJE_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (dev >= 0 && dev < 64) set[dev].store(true);
+    return GAJE_OK;
+}
+
+template <typename T, int HD, RowForm FORM>
+int launch_form(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
+    static std::atomic<bool> set[2][64];
+    const int64_t blocks = (a.prefix.items + a.keys.items) * p.n_head_kv;
     if (blocks > (int64_t)1 << 23)
         return set_error(GAJE_ERR_UNSUPPORTED, "attention over %lld tiles of rows (2^23 at most)", (long long)blocks);
-    const unsigned grid = (unsigned)blocks;
-    if (plan.bm == 16) {
-        attn_few_kernel<T, HD, 1, PREFIX><<<grid, 256, 0, s>>>(p, plan);
-    } else if (plan.bm == 32) {
-        attn_few_kernel<T, HD, FewCfg<T, HD>::NQ2, PREFIX><<<grid, 256, 0, s>>>(p, plan);
+    if (a.prefix.items) {
+        constexpr size_t lds = std::max(lds_of<T, HD, FORM>(), lds_of<T, HD, ROWS_FEW>());
+        GAJE_TRY(set_lds((const void *)attn_prefix_kernel<T, HD, FORM>, lds, set[1]));
+        attn_prefix_kernel<T, HD, FORM><<<(unsigned)blocks, 256, lds, s>>>(p, a.prefix, a.keys);
     } else {
-        const void *kernel;
-        size_t lds;
-        if constexpr (sizeof(T) == 4) {
-            kernel = (const void *)attn_split_kernel<HD, PREFIX>;
-            lds = SplitCfg<HD>::LDS;
-        } else {
-            kernel = (const void *)attn_tile_kernel<T, HD, PREFIX>;
-            lds = TileCfg<T, HD>::LDS;
-        }
-        static std::atomic<bool> set[64];
-        int dev = 0;
-        GAJE_HIP_CHECK(hipGetDevice(&dev));
-        if (dev < 0 || dev >= 64 || !set[dev].load()) {
-            GAJE_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-            if (dev >= 0 && dev < 64) set[dev].store(true);
-        }
-        if constexpr (sizeof(T) == 4) attn_split_kernel<HD, PREFIX><<<grid, 256, lds, s>>>(p, plan);
-        else attn_tile_kernel<T, HD, PREFIX><<<grid, 256, lds, s>>>(p, plan);
+        constexpr size_t lds = lds_of<T, HD, FORM>();
+        GAJE_TRY(set_lds((const void *)attn_kernel<T, HD, FORM>, lds, set[0]));
+        attn_kernel<T, HD, FORM><<<(unsigned)blocks, 256, lds, s>>>(p, a.keys);
     }
     GAJE_HIP_CHECK(hipGetLastError());
     return GAJE_OK;
 }
 
-template <typename T, bool PREFIX>
-int launch_part(const ServeAttnParams &p, const TilePlan &plan, hipStream_t s) {
-    const int hd = hd_class(p.head_dim);
-    if (hd == 64) return launch_tiles<T, 64, PREFIX>(p, plan, s);
-    if (hd == 128) return launch_tiles<T, 128, PREFIX>(p, plan, s);
-    return launch_tiles<T, 256, PREFIX>(p, plan, s);
+template <typename T, int HD>
+int launch_head(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
+    const int bm = a.prefix.items ? a.prefix.bm : a.keys.bm;
+    if (bm == 16) return launch_form<T, HD, ROWS_FEW>(p, a, s);
+    return launch_form<T, HD, ROWS_TILE>(p, a, s);
 }
 
 template <typename T>
 int launch_typed(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
-    if (a.prefix.items) GAJE_TRY((launch_part<T, true>(p, a.prefix, s)));
-    GAJE_TRY((launch_part<T, false>(p, a.keys, s)));
+    const int hd = hd_class(p.head_dim);
+    if (hd == 64) GAJE_TRY((launch_head<T, 64>(p, a, s)));
+    else if (hd == 128) GAJE_TRY((launch_head<T, 128>(p, a, s)));
+    else GAJE_TRY((launch_head<T, 256>(p, a, s)));
     if (a.parts) {
         const dim3 grid((unsigned)((p.T + 3) / 4), (unsigned)p.n_head);
         if (p.head_dim <= 64) attn_join_kernel<T, 16><<<grid, 256, 0, s>>>(p, a.keys, a.prefix);

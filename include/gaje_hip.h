@@ -329,7 +329,7 @@ int gaje_hip_kv_append(const gaje_hip_kv_pages *c, int64_t layer, int source_dty
  * h / (n_head / n_head_kv).  out row: softmax(scale q.k) v, written in the type.
  * seq_off: device [n_seq + 1], ascending; empty sequences are allowed, rows past
  * seq_off[n_seq] of out are left as they were.  NaN and infinities reach only the
- * rows that see them.  head_dim a multiple of 8 up to 256, scale > 0 and finite,
+ * rows that see them.  head_dim a multiple of 8 up to 256, scale > 0 and at most 1e30,
  * q, k, v, out 16-byte aligned with leading dimensions that are multiples of 8, up to 2^21.
  * `workspace`: the matching _workspace() bytes, 16-byte aligned; nothing is kept
  * in it between calls, and calls that share one must not overlap. */
