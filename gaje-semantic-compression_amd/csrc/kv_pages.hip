@@ -267,7 +267,15 @@ __device__ __forceinline__ void copy_pages(const gaje_hip_kv_pages &c, const int
         char *pool = (char *)(i & 1 ? c.v : c.k) + layer * c.n_pages * page_bytes;
         const char *from = pool + src[copy] * page_bytes;
         char *to = pool + dst[copy] * page_bytes;
-        for (int64_t b = threadIdx.x * 16; b < page_bytes; b += 256 * 16) *(vu4 *)(to + b) = *(const vu4 *)(from + b);
+        // four pieces of a thread in flight
+        for (int64_t b = threadIdx.x * 16; b < page_bytes; b += 4 * 256 * 16) {
+            vu4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = *(const vu4 *)(from + min(b + u * 4096, page_bytes - 16));
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (b + u * 4096 < page_bytes) *(vu4 *)(to + b + u * 4096) = x[u];
+        }
     }
 }
 // The new arrays, or the old ones where the plan failed, and the copies.

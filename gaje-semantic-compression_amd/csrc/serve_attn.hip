@@ -29,10 +29,10 @@ typedef __bf16 vb8 __attribute__((ext_vector_type(8)));
 
 // What a row outside the sequence, a padded dimension and a page outside the pool
 // read: loads are redirected here instead of being skipped.
-__device__ const vu4 zero_piece = {0, 0, 0, 0};
+__device__ const vu4 zero_piece[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 typedef const __attribute__((address_space(1))) vu4 *gvu4;
 typedef const __attribute__((address_space(1))) char *gchar;
-__device__ __forceinline__ gvu4 piece(const void *p, bool ok) { return ok ? (gvu4)(uintptr_t)p : (gvu4)(uintptr_t)&zero_piece; }
+__device__ __forceinline__ gvu4 piece(const void *p, bool ok) { return ok ? (gvu4)(uintptr_t)p : (gvu4)(uintptr_t)zero_piece; }
 
 // 16 x 16 and 32 x 32 products of 16-bit operands, eight of a lane's at a time.
 template <typename T>
@@ -374,8 +374,10 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
     int rows_at[2];
 #pragma unroll
     for (int a = 0; a < 2; ++a) rows_at[a] = is_v ? (set >> 1) * 16 + (set & 1) * 4 + 8 * a : set * 8 + 4 * a;
-    const char *const base = (const char *)((const T *)(is_v ? p.v : p.k) + (int64_t)g * hd) + pc * 16;
-    const uint32_t ld = (uint32_t)(is_v ? p.ldv : p.ldk) * sizeof(T);
+    // (a padded dimension's thread reads zeros with a step of 0)
+    const bool in = pc * 8 < hd;
+    const char *const base = in ? (const char *)((const T *)(is_v ? p.v : p.k) + (int64_t)g * hd) + pc * 16 : (const char *)zero_piece;
+    const uint32_t ld = in ? (uint32_t)(is_v ? p.ldv : p.ldk) * sizeof(T) : 0;
     vu4 rg[8];
     int ids[2];
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
@@ -397,13 +399,13 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
                 at[a] = base + (int64_t)(q.row0 + k0) * ld + (uint32_t)rows_at[a] * ld;
             }
         }
-        if (k0 + BN <= kb1 && hd == HD && __all(held[0] & held[1])) {
+        if (k0 + BN <= kb1 && __all(held[0] & held[1])) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) rg[i] = *(gvu4)(uintptr_t)(at[i >> 2] + (i & 3) * ld);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                rg[i] = *piece(at[i >> 2] + (i & 3) * ld, (pc * 8 < hd) & (k0 + rows_at[i >> 2] + (i & 3) < kb1) & held[i >> 2]);
+                rg[i] = *piece(at[i >> 2] + (i & 3) * ld, (k0 + rows_at[i >> 2] + (i & 3) < kb1) & held[i >> 2]);
         }
     };
     char *const Kw = lds + ((set >> 2) * C::PCS + pc) * C::KROW + (set & 3) * 128;
@@ -642,9 +644,11 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
     // K: rows tid / PCS (and 256 / PCS on), dimensions 8 (tid % PCS); V: dimensions VD (tid % 64) of
     // the wave's eight keys 4 w + 0..3, 16 + 4 w + 0..3
     const int kpc = tid % C::PCS, krow = tid / C::PCS, vd = lane * C::VD;
-    const char *const Kg = (const char *)((const float *)p.k + (int64_t)g * hd + kpc * 8);
-    const char *const Vg = (const char *)((const float *)p.v + (int64_t)g * hd + vd);
-    const uint32_t ldk = (uint32_t)p.ldk * 4, ldv = (uint32_t)p.ldv * 4;
+    // (a padded dimension's thread reads zeros with a step of 0)
+    const bool kin = kpc * 8 < hd, vin = vd < hd;
+    const char *const Kg = kin ? (const char *)((const float *)p.k + (int64_t)g * hd + kpc * 8) : (const char *)zero_piece;
+    const char *const Vg = vin ? (const char *)((const float *)p.v + (int64_t)g * hd + vd) : (const char *)zero_piece;
+    const uint32_t ldk = kin ? (uint32_t)p.ldk * 4 : 0, ldv = vin ? (uint32_t)p.ldv * 4 : 0;
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
     const int page_mask = (1 << p.page_shift) - 1;
     vu4 kr[C::KU][2];
@@ -686,7 +690,7 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
             va[a] = row_of(Vg, ldv, vid[a], k0 + 16 * a + 4 * wave);
             held = held & (!p.table | ((uint32_t)vid[a] < (uint32_t)p.n_pages));
         }
-        if (hd == HD && k0 + BN <= kb1 && __all(held)) {
+        if (k0 + BN <= kb1 && __all(held)) {
 #pragma unroll
             for (int n = 0; n < C::KU; ++n) kr[n][0] = *(gvu4)(uintptr_t)ka[n], kr[n][1] = *(gvu4)(uintptr_t)(ka[n] + 16);
 #pragma unroll
@@ -695,13 +699,13 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
         }
 #pragma unroll
         for (int n = 0; n < C::KU; ++n) {
-            const bool ok = (k0 + krow + n * (256 / C::PCS) < kb1) & (kpc * 8 < hd) & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
+            const bool ok = (k0 + krow + n * (256 / C::PCS) < kb1) & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
             kr[n][0] = *piece(ka[n], ok);
             kr[n][1] = *piece(ka[n] + 16, ok);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            take_v(vr[i], piece(va[i >> 2] + (i & 3) * ldv, (k0 + (i >> 2) * 16 + 4 * wave + (i & 3) < kb1) & (vd < hd) &
+            take_v(vr[i], piece(va[i >> 2] + (i & 3) * ldv, (k0 + (i >> 2) * 16 + 4 * wave + (i & 3) < kb1) &
                                                                 (!p.table | ((uint32_t)vid[i >> 2] < (uint32_t)p.n_pages))));
     };
     char *const Kw = lds + ((krow >> 4) * C::PCS + kpc) * C::KCH + (krow & 15) * 16;
@@ -1254,6 +1258,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, TileP
     const int s = seq_of_row(p, (int)t);
     if (s < 0) return;
     const Seq q = seq_at(p, s);
+    if (t < q.row0 || t >= q.row0 + q.rows) return;  // (offsets that do not ascend)
     // the parts that its tiles wrote
     const int tile = (int)((((int64_t)t - q.row0) * group + h % group) / keys.bm);
     const int kend = tile_end<false>(p, q, tile, keys.bm, group), from = min(keys.key0, kend) & ~31;

@@ -269,9 +269,9 @@ enum { GAJE_DTYPE_F32 = 0, GAJE_DTYPE_F16 = 1, GAJE_DTYPE_BF16 = 2 };
  * len[s] positions, position p in row p % page of page table[s][p / page].
  * ref[i] counts the table entries that name page i (0: free).  head_dim is a
  * multiple of 8 up to 256; k and v are 16-byte aligned; max_pages * page is 2^24 at
- * most.  No kernel follows a
- * page id outside 0..n_pages-1: rows there read as zeros and are not written.
- * len is taken as at most max_pages * page, and at least 0. */
+ * most.  No kernel follows a page id outside 0..n_pages-1: rows there read as
+ * zeros and are not written.  len is taken as at least 0 and at most max_pages *
+ * page.  All buffers belong to the current device. */
 typedef struct {
     void *k, *v;                 /* [n_layer][n_pages][page][n_head_kv][head_dim] of dtype */
     int32_t *table;              /* [n_seq][max_pages] page ids, -1 past a sequence's last  */
@@ -292,9 +292,9 @@ typedef struct {
  * Results go to new_table [n_seq][max_pages] (-1 past the last page), new_len,
  * new_ref, which must not overlap the cache's own arrays: the caller swaps
  * them in.  status[0] (device) gets 0, or the sum of 1 (a source outside
- * -1..n_seq-1), 2 (a length below 0 or past max_pages * page), 4 (too few free
- * pages), 8 (a table entry in use outside the pool): then the new arrays are
- * the old ones and no page is copied.  All arrays are device memory and nothing
+ * -1..n_seq-1), 2 (a length below 0 or past max_pages * page), 8 (a table entry
+ * in use outside the pool), or else 4 (too few free pages): then the new arrays
+ * are the old ones and no page is copied.  All arrays are device memory and nothing
  * is read on the host, so that the call can be captured in a graph.
  * `workspace`: gaje_hip_kv_workspace(c) bytes, 16-byte aligned; calls that share
  * one must not overlap.  n_pages up to 2^26, n_seq up to 2^20. */
@@ -328,8 +328,9 @@ int gaje_hip_kv_append(const gaje_hip_kv_pages *c, int64_t layer, int source_dty
  * one fused product), row i sees rows seq_off[s]..i.  Query head h reads K/V head
  * h / (n_head / n_head_kv).  out row: softmax(scale q.k) v, written in the type.
  * seq_off: device [n_seq + 1], ascending; empty sequences are allowed, rows past
- * seq_off[n_seq] of out are left as they were.  NaN and infinities reach only the
- * rows that see them.  head_dim a multiple of 8 up to 256, scale > 0 and at most 1e30,
+ * seq_off[n_seq] of out are left as they were; out overlaps no input.  NaN and
+ * infinities reach only the rows that see them (a row whose result is no number is
+ * computed again key by key: correct, and slow if there are many).  head_dim a multiple of 8 up to 256, scale > 0 and at most 1e30,
  * q, k, v, out 16-byte aligned with leading dimensions that are multiples of 8, up to 2^21.
  * `workspace`: the matching _workspace() bytes, 16-byte aligned; nothing is kept
  * in it between calls, and calls that share one must not overlap. */

@@ -575,3 +575,100 @@ def test_same_bits_again(ops):
     _, h = device_cache(ops, c)
     q = normal((3, H * hd), "f32", 4).cuda()
     assert torch.equal(run_paged(ops, h, q, [1] * 3, H, 0.1), run_paged(ops, h, q, [1] * 3, H, 0.1))
+
+
+def guarded(nbytes):
+    """A workspace of exactly nbytes (a multiple of 4), and the words behind it."""
+    t = torch.full((nbytes // 4 + 64,), 7.0, device="cuda")
+
+    class W:
+        ptr, buf = t.data_ptr(), t
+    W.nbytes = nbytes
+    return W, t[nbytes // 4:]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("H,G,hd,rows,seqs,length", [(14, 2, 64, 1, 5, 3000), (6, 2, 128, 9, 2, 2500), (3, 3, 24, 1, 70, 300)])
+def test_workspaces_are_kept_to(ops, dtype, H, G, hd, rows, seqs, length):
+    """Calls write no further than their _workspace() bytes."""
+    c = R.Cache([length - 7 * i for i in range(seqs)] if length > 7 * seqs else [length] * seqs, 16, G, hd, dtype, spare=80, max_pages=256)
+    t, h = device_cache(ops, c)
+    q = normal((rows * seqs, H * hd), dtype, 3).cuda()
+    out, off = torch.empty_like(q), offsets([rows] * seqs)
+    ws, tail = guarded(ops.attention_paged_workspace(h, rows * seqs, H) // 4 * 4)
+    ops.attention_paged(Buf(q), H * hd, h, 0, Buf(off), rows * seqs, H, 0.1, Buf(out), H * hd, ws)
+    assert bool((tail == 7).all())
+    check_paged(c, q, out, [rows] * seqs, H, 0.1)
+    ws, tail = guarded(ops.attention_prefix_workspace(h, 100, H) // 4 * 4)
+    ops.attention_prefix(Buf(q), H * hd, h, 0, Buf(t["table"]), 100, H, 0.1, Buf(out), H * hd, ws)
+    assert bool((tail == 7).all())
+    x = normal((rows * seqs, (H + 2 * G) * hd), dtype, 4).cuda()
+    ws, tail = guarded(ops.attention_packed_workspace(rows * seqs, seqs, H, G, hd) // 4 * 4)
+    ops.attention_packed(Buf(x), x.shape[1], Buf(x, H * hd), x.shape[1], Buf(x, (H + G) * hd), x.shape[1], Buf(off), seqs, rows * seqs, H,
+                         G, hd, 0.1, Buf(out), H * hd, ws, dtype=dtype)
+    assert bool((tail == 7).all())
+    check_packed(x, out, [rows] * seqs, H, G, hd, 0.1, dtype)
+    ws, tail = guarded(ops.kv_workspace(h) // 4 * 4)
+    new, status = {k: torch.empty_like(t[k]) for k in ("table", "length", "ref")}, ints([9])
+    ops.kv_update(h, Buf(new["table"]), Buf(new["length"]), Buf(new["ref"]), Buf(status), ws, add=Buf(ints([1] * seqs)))
+    assert int(status.cpu()[0]) == 0 and bool((tail == 7).all())
+    ops.kv_compact(h, Buf(new["table"]), Buf(new["ref"]), Buf(status), ws)
+    torch.cuda.synchronize()
+    assert bool((tail == 7).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_many_sequences(ops, dtype):
+    """Thousands of short ones, and a few thousand rows over a few of many slots."""
+    rows = [(i * 7) % 4 for i in range(3000)]
+    H, G, hd = 4, 2, 32
+    x = normal((sum(rows), (H + 2 * G) * hd), dtype, 5).cuda()
+    check_packed(x, run_packed(ops, x, rows, H, G, hd, 0.2), rows, H, G, hd, 0.2, dtype)
+    rows = [0] * 200 + [90] + [0] * 150 + [300] + [0] * 100
+    x = normal((sum(rows), (H + 2 * G) * hd), dtype, 6).cuda()
+    check_packed(x, run_packed(ops, x, rows, H, G, hd, 0.2), rows, H, G, hd, 0.2, dtype)
+
+
+def test_two_calls_at_once(ops):
+    """Calls on two streams, each with a workspace of its own."""
+    H, G, hd = 6, 2, 64
+    c = R.Cache([2000, 900, 3], 16, G, hd, "f16", max_pages=256)
+    _, h = device_cache(ops, c)
+    q = [normal((3, H * hd), "f16", s).cuda() for s in (1, 2)]
+    want = [run_paged(ops, h, x, [1] * 3, H, 0.1) for x in q]
+    streams, out, off = [torch.cuda.Stream() for _ in q], [torch.empty_like(x) for x in q], offsets([1] * 3)
+    ws = [space(ops.attention_paged_workspace(h, 3, H)) for _ in q]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, o, w, s in zip(q, out, ws, streams):
+            ops.attention_paged(Buf(x), H * hd, h, 0, Buf(off), 3, H, 0.1, Buf(o), H * hd, Buf(w), stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1e-38, 1e-6, 20.0])
+def test_scales(ops, dtype, scale):
+    """Scales that make all weights alike, and that leave one."""
+    rows, H, G, hd = [70, 300], 4, 2, 64
+    x = normal((sum(rows), (H + 2 * G) * hd), dtype, seed=5).cuda()
+    check_packed(x, run_packed(ops, x, rows, H, G, hd, scale), rows, H, G, hd, scale, dtype)
+    c = R.Cache([900, 40], 16, G, hd, dtype)
+    _, h = device_cache(ops, c)
+    q = normal((2, H * hd), dtype, 3).cuda()
+    check_paged(c, q, run_paged(ops, h, q, [1, 1], H, scale), [1, 1], H, scale)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scores_of_minus_infinity(ops, dtype):
+    """Keys whose score is -inf have no weight; a row that sees only such keys is no number, as a
+    softmax of them is; values past f32's parts are what they are."""
+    H, G, hd, n = 2, 1, 64, 200
+    x = normal((n, (H + 2 * G) * hd), dtype, 7).abs()
+    x[:, :H * hd] += 0.5                       # positive queries
+    x[:40, H * hd:(H + 1) * hd] = -math.inf    # and keys of -inf: every score with them is -inf
+    out = run_packed(ops, x.cuda(), [n], H, G, hd, 0.1).cpu().reshape(n, H, hd)
+    assert bool(torch.isnan(out[:40].float()).all())
+    q, k, v = (x[:, a * hd:b * hd].reshape(n, b - a, hd) for a, b in ((0, H), (H, H + G), (H + G, H + 2 * G)))
+    ref, mass, top = R.attend(q[40:], k[40:], v[40:], 0, 0.1)
+    close(out[40:], ref, R.bound(dtype, ref, mass, top, hd, n))
