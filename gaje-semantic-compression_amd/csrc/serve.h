@@ -32,8 +32,8 @@ struct ServeAttnParams {
     // (one row per sequence, seq_off null)
     const int32_t *prefix_table;  // null: none
     int64_t prefix_len;
-    // keys per part, then partial results: [n_part][T][n_head] (maximum, sum) and [n_part][T][n_head][head_dim]
-    int32_t *part_size;
+    // parts of each row's own keys, [T][n_head], and partial results: [n_part][T][n_head] (maximum, sum) and [n_part][T][n_head][head_dim]
+    int32_t *parts;
     float2 *part_ml;
     float *part_o;
 };

@@ -228,10 +228,10 @@ __device__ __forceinline__ int tile_end(const ServeAttnParams &p, const Seq &q, 
 // What a workgroup does: part `part` of a tile's keys, `size` keys each.
 struct Item {
     Seq q;
-    int tile, part, size;
+    int g, tile, part, size;  // g: the K/V head
 };
 
-// Item b of a K/V head.  A sequence has ceil(rows group / bm) tiles, the ones over the
+// The item of a workgroup.  A sequence has ceil(rows group / bm) tiles, the ones over the
 // longest contexts first, and as many parts as its longest tile needs (a workgroup past a
 // shorter tile's end has nothing to do).  Every wave looks at all sequences, 64 at a time:
 // once for the part size, if the keys are cut at all, once for its item.
@@ -239,14 +239,18 @@ struct Item {
 // item takes up to 70 us, and one begun last ends last: 24 prompts of up to 2000 tokens, 12 heads
 // of 128, bf16, 153 -> 150 us).
 template <bool PREFIX, bool LONG_FIRST>
-__device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePlan &plan, int b, int group, Item &it) {
+__device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePlan &plan, int block, int group, Item &it) {
     if constexpr (PREFIX) {
+        const int keys = plan.splits * p.n_head_kv, at = block % keys;
         it.q = Seq{0, 0, 0, 0};
-        it.tile = b / plan.splits;
-        it.part = b % plan.splits;
+        it.g = at % p.n_head_kv;
+        it.part = at / p.n_head_kv;
+        it.tile = block / keys;
         it.size = plan.size;
         return true;
     }
+    const int b = block / p.n_head_kv;
+    it.g = block % p.n_head_kv;
     const int lane = threadIdx.x & 63, from = plan.key0 & ~31, n_seq = (int)p.n_seq, shift = __builtin_ctz(plan.bm);
     Seq q;
     int tiles, cut;  // of sequence s0 + lane; cut: keys to cut into parts
@@ -333,6 +337,14 @@ __device__ __forceinline__ Row row_at(const ServeAttnParams &p, const Seq &q, in
     return w;
 }
 
+// What the join needs to know of a row, from the first part of its own keys: how many parts
+// those have; 0: the result is whole; negative: it sees no key.
+__device__ __forceinline__ void tell_parts(const ServeAttnParams &p, const TilePlan &plan, const Item &it, const Row &row, int keys, bool whole) {
+    if (plan.part0 < 0 || it.part > 0 || !row.valid) return;
+    const int n = whole ? 0 : max((keys - 1) / it.size + 1, 1);
+    p.parts[row.t * p.n_head + row.head] = row.lim >= 0 ? n : -n;
+}
+
 template <typename T>
 __device__ __forceinline__ void store_row(const ServeAttnParams &p, int64_t t, int head, int part, bool whole, bool seen, float m,
                                           float l, const float (&o)[4]) {
@@ -357,12 +369,11 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
     constexpr int BM = 128, BN = C::BN, NB = BN / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, l32 = lane & 31;
-    const int group = p.n_head / p.n_head_kv, g = block % p.n_head_kv, hd = p.head_dim;
+    const int group = p.n_head / p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX, true>(p, plan, block / p.n_head_kv, group, it)) return;
-    if (!PREFIX && block == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    if (!find_item<PREFIX, true>(p, plan, block, group, it)) return;
     const Seq q = it.q;
-    const int tile = it.tile;
+    const int g = it.g, tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
     const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
@@ -432,6 +443,7 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
         load_ids(kb0 + BN);
     }
     const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 32 + l32, group, g);
+    if (!PREFIX && half == 0) tell_parts(p, plan, it, row, kend, whole);
     // this wave's rows: the largest and the smallest last key
     int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
 #pragma unroll
@@ -631,12 +643,11 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
     constexpr int BM = C::BM, BN = C::BN;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g4 = lane >> 4;
-    const int group = p.n_head / p.n_head_kv, g = block % p.n_head_kv, hd = p.head_dim;
+    const int group = p.n_head / p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX, true>(p, plan, block / p.n_head_kv, group, it)) return;
-    if (!PREFIX && block == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    if (!find_item<PREFIX, true>(p, plan, block, group, it)) return;
     const Seq q = it.q;
-    const int tile = it.tile;
+    const int g = it.g, tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group);
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend);
     const int part = plan.part0 + it.part, kb0 = min(it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
@@ -746,6 +757,7 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
         load_ids(kb0 + BN);
     }
     const Row row = row_at<PREFIX>(p, q, tile * BM + wave * 16 + l16, group, g);
+    if (!PREFIX && g4 == 0) tell_parts(p, plan, it, row, kend, whole);
     int lim_hi = row.lim, lim_lo = row.valid ? row.lim : INT32_MAX;
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) {
@@ -934,12 +946,11 @@ __device__ __forceinline__ void attend_few(const ServeAttnParams &p, const TileP
     auto &odd = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g4 = lane >> 4;
-    const int group = p.n_head / p.n_head_kv, g = block % p.n_head_kv, hd = p.head_dim;
+    const int group = p.n_head / p.n_head_kv, hd = p.head_dim;
     Item it;
-    if (!find_item<PREFIX, false>(p, plan, block / p.n_head_kv, group, it)) return;
-    if (!PREFIX && block == 0 && tid == 0 && plan.part0 >= 0) *p.part_size = it.size;
+    if (!find_item<PREFIX, false>(p, plan, block, group, it)) return;
     const Seq q = it.q;
-    const int tile = it.tile;
+    const int g = it.g, tile = it.tile;
     const int kend = tile_end<PREFIX>(p, q, tile, BM, group), key0 = min(plan.key0, kend), from = key0 & ~31;
     const bool whole = plan.part0 < 0 || (plan.alone && it.size >= kend - from);
     const int part = plan.part0 + it.part, kb0 = min(from + it.part * it.size, kend), kb1 = min(kb0 + it.size, kend);
@@ -1035,6 +1046,7 @@ __device__ __forceinline__ void attend_few(const ServeAttnParams &p, const TileP
     vu4 qf[C::STEPS];
     {
         const Row row = row_at<PREFIX>(p, q, tile * BM + l16, group, g);
+        if (!PREFIX && tid < 16) tell_parts(p, plan, it, row, kend - from, whole);
         lim = lim_hi = row.lim;
         lim_lo = row.valid ? lim : INT32_MAX;
         const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
@@ -1251,21 +1263,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_prefix_kernel(Ser
 template <typename T, int LPP>
 __global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, TilePlan keys, TilePlan prefix) {
     constexpr int SIDE = WAVE / LPP;
-    const int lane = threadIdx.x & 63, hd = p.head_dim, h = blockIdx.y, group = p.n_head / p.n_head_kv;
+    const int lane = threadIdx.x & 63, hd = p.head_dim, h = blockIdx.y;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= p.T) return;
-    const int size = *p.part_size;
-    const int s = seq_of_row(p, (int)t);
-    if (s < 0) return;
-    const Seq q = seq_at(p, s);
-    if (t < q.row0 || t >= q.row0 + q.rows) return;  // (offsets that do not ascend)
-    // the parts that its tiles wrote
-    const int tile = (int)((((int64_t)t - q.row0) * group + h % group) / keys.bm);
-    const int kend = tile_end<false>(p, q, tile, keys.bm, group), from = min(keys.key0, kend) & ~31;
-    if (keys.alone && size >= kend - from) return;  // written whole
-    const int np = prefix.items ? prefix.splits : 0;
-    const int parts = np + max((kend - from + size - 1) / size, 1);
-    const bool seen = min(q.len - q.rows + ((int)t - q.row0) + 1, q.len) > 0;
+    const int told = p.parts[t * p.n_head + h];
+    if (p.seq_off && (t < p.seq_off[0] || t >= p.seq_off[p.n_seq])) return;  // no row of a sequence
+    if (told == 0) return;  // written whole
+    const bool seen = told > 0;
+    const int np = prefix.items ? prefix.splits : 0, parts = np + min(abs(told), keys.splits);
     const float c = p.scale * LOG2E;
     const int64_t step = p.T * p.n_head, at = t * p.n_head + h;
     auto place = [&](int i) { return (i < np ? prefix.part0 + i : keys.part0 + i - np) * step + at; };
@@ -1319,8 +1324,9 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     t.bm = avg <= 16 || key0 > 0 ? 16 : p.dtype == GAJE_DTYPE_F32 ? 64 : 128;
     t.key0 = (int32_t)key0;
     // Workgroups wanted: two for each of 256 CUs; over a prefix one, where every part costs
-    // partial results of all rows (64 sequences over 16000 keys: 29.1 against 38.2 us).
-    t.blocks = prefix ? 8 : 9;
+    // partial results of all rows (64 sequences over 16000 keys: 29.1 against 38.2 us), and beside
+    // a long one half a CU's, which leaves fewer workgroups without an item.
+    t.blocks = prefix ? 8 : key0 >= 1024 ? 7 : 9;
     // Parts of a prompt's own keys pay from 512 keys on (f32 prompts of up to 1500 tokens 67.6
     // against 75.1 us with 256, one f16 prompt of 1500 34.1 against 42.6), of a cache's from 256 (5
     // drafted tokens, f32, 37.3 against 49.4), a few rows' and a prefix's from 128.
@@ -1415,17 +1421,18 @@ int launch_typed(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
 }  // namespace
 
 int64_t serve_attn_workspace(const ServeAttnParams &p) {
-    const int64_t n = make_plan(p).parts * p.T * p.n_head;
-    return n ? n * (8 + 4 * (int64_t)p.head_dim) + 32 : 0;
+    const int64_t parts = make_plan(p).parts, rows = (p.T * p.n_head + 3) & ~(int64_t)3;
+    return parts ? rows * (parts * (8 + 4 * (int64_t)p.head_dim) + 4) : 0;
 }
 
 int launch_serve_attn(const ServeAttnParams &params, void *workspace, hipStream_t s) {
     ServeAttnParams p = params;
     const AttnPlan a = make_plan(p);
     if (!a.prefix.items) p.prefix_table = nullptr, p.prefix_len = 0;
-    p.part_size = (int32_t *)workspace;
-    p.part_ml = (float2 *)workspace + 2;
-    p.part_o = (float *)workspace + 4 + ((2 * a.parts * p.T * p.n_head + 3) & ~(int64_t)3);
+    const int64_t rows = (p.T * p.n_head + 3) & ~(int64_t)3;
+    p.part_o = (float *)workspace;
+    p.part_ml = (float2 *)(p.part_o + a.parts * p.T * p.n_head * p.head_dim);
+    p.parts = (int32_t *)(p.part_ml + a.parts * rows);
     if (p.dtype == GAJE_DTYPE_F32) return launch_typed<float>(p, a, s);
     if (p.dtype == GAJE_DTYPE_F16) return launch_typed<_Float16>(p, a, s);
     return launch_typed<__bf16>(p, a, s);
