@@ -8,14 +8,14 @@
 // was summed is rescaled when it moves.
 //
 // Three forms over the same rows and keys: attend_tile (16-bit types, 128 rows a
-// workgroup), attend_split (f32, 64 rows, on the bf16 matrix instructions) and attend_few
-// (up to 16 rows, the keys split over the waves).  The keys of a tile are cut into parts
-// where there are few tiles; attn_join_kernel joins what the parts leave.  Measured, as
-// launched in a graph:
-//   attend_tile   one prompt of 8190, 32/8 heads of 128, f16: 610 us, 900 TFLOP/s
-//   attend_split  4 prompts of 970 to 1930, 12/2 heads of 128: 258 us, 143 TFLOP/s (f32
-//                 products of a library: 154)
-//   attend_few    512 sequences of 1000 keys, 12/2 heads of 128, bf16: 97 us, 5.4 TB/s
+// workgroup), attend_tile64 (64 rows; short prompts, and f32 on the bf16 matrix
+// instructions) and attend_few (up to 16 rows, the keys split over the waves).  The keys of a
+// tile are cut into parts where there are few tiles; attn_join_kernel joins what they leave.
+// Measured, as launched in a graph:
+//   attend_tile    one prompt of 8190, 32/8 heads of 128, f16: 610 us, 900 TFLOP/s
+//   attend_tile64  4 f32 prompts of 970 to 1930, 12/2 heads of 128: 258 us, 143 TFLOP/s (f32
+//                  products of a library: 154)
+//   attend_few     512 sequences of 1000 keys, 12/2 heads of 128, bf16: 97 us, 5.4 TB/s
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -598,24 +598,32 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
     }
 }
 
-// ---- f32 tiles ----
-// f32 rows on the bf16 matrix instructions: x = x0 + x1 + x2, each the next 8 bits of the
+// ---- tiles of 64 rows ----
+// A workgroup takes 64 rows of one K/V head, 16 a wave, and the keys 32 at a time:
+// S^T = K Q^T and O^T = V^T P^T in 16 x 16 blocks, lanes as in the few-row form.  K and V are
+// staged in operand order, V transposed; one buffer, so that several workgroups of a CU fill
+// each other's waits.
+// 16-bit types: where tiles of 128 rows are too few to fill the chip.
+// f32: on the bf16 matrix instructions.  x = x0 + x1 + x2, each the next 8 bits of the
 // mantissa (cut, so that the three parts are exactly x), and x y summed from x0 y0, x0 y1,
 // x1 y0, x1 y1, x0 y2, x2 y0: what is left out is below 2^-22 of |x y|, about f32's own
-// rounding over a few products.  Six products at 16 times the rate of the f32 matrix
-// instructions; an infinity's parts are no numbers, and its rows are computed again.
-// A workgroup takes 64 rows of one K/V head, 16 a wave, and the keys 32 at a time:
-// S^T = K Q^T and O^T = V^T P^T in 16 x 16 blocks, lanes as in the few-row kernel.  K and V
-// are split on the way into LDS (operand order, V transposed); one buffer of 48 KB (128
-// dimensions), so that three workgroups of a CU fill each other's waits.
-template <int HD>
-struct SplitCfg {
+// rounding over a few products (measured against 64 bits: 4.2e-7 where f32 products give
+// 5.4e-7).  Six products at 16 times the rate of the f32 matrix instructions; an infinity's
+// parts are no numbers, and its rows are computed again.  K and V are split on the way into
+// LDS, 48 KB for 128 dimensions.
+template <typename T, int HD>
+struct Tile64Cfg {
+    static constexpr bool F32 = sizeof(T) == 4;
+    using Op = std::conditional_t<F32, __bf16, T>;     // type of the products
+    static constexpr int PL = F32 ? 3 : 1, PRODUCTS = F32 ? 6 : 1;  // planes of an operand, products of two
     static constexpr int BM = 64, BN = 32, PCS = HD / 8, STEPS = HD / 32, VT = HD / 16;
     static constexpr int VD = HD / 64;                 // dimensions of V per thread
+    static constexpr int VW = F32 ? VD : (VD + 1) / 2; // dwords of them
     static constexpr int KU = BN * PCS / 256;          // rows x 8 dimensions of K per thread
+    static constexpr int KL = F32 ? 2 : 1;             // loads of those
     static constexpr int KCH = 16 * 16 + 16;           // bytes of 16 keys' pieces, 4 banks on
     static constexpr int KP = 2 * PCS * KCH, VP = VT * 1024;  // bytes of a plane
-    static constexpr int LDS = 3 * (KP + VP);
+    static constexpr int LDS = PL * (KP + VP);
 };
 
 // The three parts of a and b, packed: a in the low halves.
@@ -630,9 +638,9 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
 }
 // the products, the smallest first
 constexpr int SPLIT_A[6] = {2, 1, 0, 1, 0, 0}, SPLIT_B[6] = {0, 1, 2, 0, 1, 0};
-template <int HD, bool PREFIX>
-__device__ __forceinline__ void attend_split(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
-    using C = SplitCfg<HD>;
+template <typename T, int HD, bool PREFIX>
+__device__ __forceinline__ void attend_tile64(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
+    using C = Tile64Cfg<T, HD>;
     constexpr int BM = C::BM, BN = C::BN;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g4 = lane >> 4;
@@ -650,13 +658,13 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
     const int kpc = tid % C::PCS, krow = tid / C::PCS, vd = lane * C::VD;
     // (a padded dimension's thread reads zeros with a step of 0)
     const bool kin = kpc * 8 < hd, vin = vd < hd;
-    const char *const Kg = kin ? (const char *)((const float *)p.k + (int64_t)g * hd + kpc * 8) : (const char *)zero_piece;
-    const char *const Vg = vin ? (const char *)((const float *)p.v + (int64_t)g * hd + vd) : (const char *)zero_piece;
-    const uint32_t ldk = kin ? (uint32_t)p.ldk * 4 : 0, ldv = vin ? (uint32_t)p.ldv * 4 : 0;
+    const char *const Kg = kin ? (const char *)((const T *)p.k + (int64_t)g * hd + kpc * 8) : (const char *)zero_piece;
+    const char *const Vg = vin ? (const char *)((const T *)p.v + (int64_t)g * hd + vd) : (const char *)zero_piece;
+    const uint32_t ldk = kin ? (uint32_t)p.ldk * sizeof(T) : 0, ldv = vin ? (uint32_t)p.ldv * sizeof(T) : 0;
     const int32_t *const pages = PREFIX ? p.prefix_table : p.table + (int64_t)q.id * p.max_pages;
     const int page_mask = (1 << p.page_shift) - 1;
-    vu4 kr[C::KU][2];
-    uint32_t vr[8][C::VD];
+    vu4 kr[C::KU][C::KL];
+    uint32_t vr[8][C::VW];
     int kid[C::KU], vid[2];
     auto load_ids = [&](int k0) {
         if (!p.table) return;
@@ -669,16 +677,18 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
         if (!p.table) return base + (int64_t)(q.row0 + pos) * ld;
         return base + (uint32_t)(pos & page_mask) * ld + (uint64_t)(uint32_t)id * (ld << p.page_shift);
     };
-    auto take_v = [&](uint32_t (&to)[C::VD], gvu4 at) {
-        if constexpr (C::VD == 4) {
+    auto take_v = [&](uint32_t (&to)[C::VW], gvu4 at) {
+        if constexpr (C::VW == 4) {
             const vu4 x = *at;
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e] = x[e];
-        } else if constexpr (C::VD == 2) {
+        } else if constexpr (C::VW == 2) {
             const vu2 x = *(const __attribute__((address_space(1))) vu2 *)at;
             to[0] = x.x, to[1] = x.y;
-        } else {
+        } else if constexpr (C::F32 || C::VD == 2) {
             to[0] = *(const __attribute__((address_space(1))) uint32_t *)at;
+        } else {
+            to[0] = *(const __attribute__((address_space(1))) uint16_t *)at;
         }
     };
     auto load_tile = [&](int k0) {
@@ -696,7 +706,9 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
         }
         if (k0 + BN <= kb1 && __all(held)) {
 #pragma unroll
-            for (int n = 0; n < C::KU; ++n) kr[n][0] = *(gvu4)(uintptr_t)ka[n], kr[n][1] = *(gvu4)(uintptr_t)(ka[n] + 16);
+            for (int n = 0; n < C::KU; ++n)
+#pragma unroll
+                for (int x = 0; x < C::KL; ++x) kr[n][x] = *(gvu4)(uintptr_t)(ka[n] + 16 * x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) take_v(vr[i], (gvu4)(uintptr_t)(va[i >> 2] + (i & 3) * ldv));
             return;
@@ -704,8 +716,8 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
 #pragma unroll
         for (int n = 0; n < C::KU; ++n) {
             const bool ok = (k0 + krow + n * (256 / C::PCS) < kb1) & (!p.table | ((uint32_t)kid[n] < (uint32_t)p.n_pages));
-            kr[n][0] = *piece(ka[n], ok);
-            kr[n][1] = *piece(ka[n] + 16, ok);
+#pragma unroll
+            for (int x = 0; x < C::KL; ++x) kr[n][x] = *piece(ka[n] + 16 * x, ok);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -713,37 +725,45 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
                                                                 (!p.table | ((uint32_t)vid[i >> 2] < (uint32_t)p.n_pages))));
     };
     char *const Kw = lds + ((krow >> 4) * C::PCS + kpc) * C::KCH + (krow & 15) * 16;
-    char *const Vw = lds + 3 * C::KP + (lane >> 4) * C::VD * 1024 + (wave * 16 + l16) * 16;
+    char *const Vw = lds + C::PL * C::KP + (lane >> 4) * C::VD * 1024 + (wave * 16 + l16) * 16;
     auto store_tile = [&]() {
 #pragma unroll
         for (int n = 0; n < C::KU; ++n) {
-            vu4 w[3];
+            vu4 w[C::PL];
+            if constexpr (C::F32) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t u[3];
-                split3(__uint_as_float(kr[n][x >> 1][(x & 1) * 2]), __uint_as_float(kr[n][x >> 1][(x & 1) * 2 + 1]), u);
-                w[0][x] = u[0], w[1][x] = u[1], w[2][x] = u[2];
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t u[3];
+                    split3(__uint_as_float(kr[n][x >> 1][(x & 1) * 2]), __uint_as_float(kr[n][x >> 1][(x & 1) * 2 + 1]), u);
+                    w[0][x] = u[0], w[1][x] = u[1], w[2][x] = u[2];
+                }
+            } else {
+                w[0] = kr[n][0];
             }
             // (16 rows on where a block of keys has fewer threads)
             char *to = Kw + (256 / C::PCS >= 16 ? n * (256 / C::PCS / 16) * C::PCS * C::KCH : (n & 1) * (256 / C::PCS) * 16 + (n >> 1) * C::PCS * C::KCH);
 #pragma unroll
-            for (int y = 0; y < 3; ++y) *(vu4 *)(to + y * C::KP) = w[y];
+            for (int y = 0; y < C::PL; ++y) *(vu4 *)(to + y * C::KP) = w[y];
         }
 #pragma unroll
         for (int e = 0; e < C::VD; ++e) {
-            vu4 w[3];
+            vu4 w[C::PL];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                uint32_t u[3];
-                split3(__uint_as_float(vr[2 * x][e]), __uint_as_float(vr[2 * x + 1][e]), u);
-                w[0][x] = u[0], w[1][x] = u[1], w[2][x] = u[2];
+                if constexpr (C::F32) {
+                    uint32_t u[3];
+                    split3(__uint_as_float(vr[2 * x][e]), __uint_as_float(vr[2 * x + 1][e]), u);
+                    w[0][x] = u[0], w[1][x] = u[1], w[2][x] = u[2];
+                } else {
+                    w[0][x] = __builtin_amdgcn_perm(vr[2 * x + 1][e >> 1], vr[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                }
             }
 #pragma unroll
-            for (int y = 0; y < 3; ++y) *(vu4 *)(Vw + e * 1024 + y * C::VP) = w[y];
+            for (int y = 0; y < C::PL; ++y) *(vu4 *)(Vw + e * 1024 + y * C::VP) = w[y];
         }
     };
 
-    vu4 qf[3][C::STEPS];
+    vu4 qf[C::PL][C::STEPS];
     if (kb0 < kb1) {
         load_ids(kb0);
         load_tile(kb0);
@@ -759,18 +779,24 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
     }
     lim_hi = __builtin_amdgcn_readfirstlane(lim_hi), lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
     {
-        const float *Q = (const float *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
+        const T *Q = (const T *)p.q + row.t * p.ldq + (int64_t)row.head * hd;
 #pragma unroll
         for (int j = 0; j < C::STEPS; ++j) {
             const int e = (4 * j + g4) * 8;
             const bool ok = row.valid && e < hd;
-            const vu4 a = *piece(Q + e, ok), b = *piece(Q + e + 4, ok);
+            const vu4 a = *piece(Q + e, ok);
+            if constexpr (C::F32) {
+                const vu4 b = *piece(Q + e + 4, ok);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t u[3];
-                const vu4 &h = x < 2 ? a : b;
-                split3(__uint_as_float(h[(x & 1) * 2]), __uint_as_float(h[(x & 1) * 2 + 1]), u);
-                qf[0][j][x] = u[0], qf[1][j][x] = u[1], qf[2][j][x] = u[2];
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t u[3];
+                    const vu4 &h = x < 2 ? a : b;
+                    split3(__uint_as_float(h[(x & 1) * 2]), __uint_as_float(h[(x & 1) * 2 + 1]), u);
+                    qf[0][j][x] = u[0], qf[1][j][x] = u[1], qf[2][j][x] = u[2];
+                }
+            } else {
+                qf[0][j] = a;
+                asm volatile("" : "+v"(qf[0][j]));  // (waited for here, as in the tiles of 128 rows)
             }
         }
     }
@@ -779,7 +805,7 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
     vf4 o[C::VT];
 #pragma unroll
     for (int t = 0; t < C::VT; ++t) o[t] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
-    const char *const Kr = lds + g4 * C::KCH + l16 * 16, *const Vr = lds + 3 * C::KP + lane * 16;
+    const char *const Kr = lds + g4 * C::KCH + l16 * 16, *const Vr = lds + C::PL * C::KP + lane * 16;
     for (int k0 = kb0; k0 < kb1; k0 += BN) {
         store_tile();
         __syncthreads();
@@ -791,15 +817,15 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
             vf4 s[2] = {vf4{0.0f, 0.0f, 0.0f, 0.0f}, vf4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int j = 0; j < C::STEPS; ++j) {
-                vu4 k[2][3];
+                vu4 k[2][C::PL];
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int y = 0; y < 3; ++y) k[b][y] = *(const vu4 *)(Kr + y * C::KP + (b * C::PCS + 4 * j) * C::KCH);
+                    for (int y = 0; y < C::PL; ++y) k[b][y] = *(const vu4 *)(Kr + y * C::KP + (b * C::PCS + 4 * j) * C::KCH);
 #pragma unroll
-                for (int x = 0; x < 6; ++x)
+                for (int x = 6 - C::PRODUCTS; x < 6; ++x)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) s[b] = mfma16<__bf16>(k[b][SPLIT_A[x]], qf[SPLIT_B[x]][j], s[b]);
+                    for (int b = 0; b < 2; ++b) s[b] = mfma16<typename C::Op>(k[b][SPLIT_A[x]], qf[SPLIT_B[x]][j], s[b]);
             }
             if (k0 + BN - 1 > lim_lo) {
                 int lim = row.lim - k0 - 4 * g4;
@@ -828,28 +854,34 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
                 m = to;
             }
             const float base = m == -INFINITY ? 0.0f : m * c;
-            vu4 w[3];
+            vu4 w[C::PL];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                     const float e0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -base)), e1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], c, -base));
                     l += e0 + e1;
-                    uint32_t u[3];
-                    split3(e0, e1, u);
-                    w[0][b * 2 + i / 2] = u[0], w[1][b * 2 + i / 2] = u[1], w[2][b * 2 + i / 2] = u[2];
+                    if constexpr (C::F32) {
+                        uint32_t u[3];
+                        split3(e0, e1, u);
+                        w[0][b * 2 + i / 2] = u[0], w[1][b * 2 + i / 2] = u[1], w[2][b * 2 + i / 2] = u[2];
+                    } else {
+                        union { T e[2]; uint32_t u; } x;
+                        x.e[0] = (T)e0, x.e[1] = (T)e1;
+                        w[0][b * 2 + i / 2] = x.u;
+                    }
                 }
 #pragma unroll
             for (int t = 0; t < C::VT; t += 2) {
-                vu4 v[2][3];
+                vu4 v[2][C::PL];
 #pragma unroll
                 for (int z = 0; z < 2; ++z)
 #pragma unroll
-                    for (int y = 0; y < 3; ++y) v[z][y] = *(const vu4 *)(Vr + y * C::VP + (t + z) * 1024);
+                    for (int y = 0; y < C::PL; ++y) v[z][y] = *(const vu4 *)(Vr + y * C::VP + (t + z) * 1024);
 #pragma unroll
-                for (int x = 0; x < 6; ++x)
+                for (int x = 6 - C::PRODUCTS; x < 6; ++x)
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) o[t + z] = mfma16<__bf16>(v[z][SPLIT_A[x]], w[SPLIT_B[x]], o[t + z]);
+                    for (int z = 0; z < 2; ++z) o[t + z] = mfma16<typename C::Op>(v[z][SPLIT_A[x]], w[SPLIT_B[x]], o[t + z]);
             }
         }
         __syncthreads();
@@ -871,7 +903,8 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
         const bool seen = row.lim >= 0;
         const int64_t at = ((int64_t)part * p.T + row.t) * p.n_head + row.head;
         const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
-        float *to = whole ? (float *)p.out + row.t * p.ldo + (int64_t)row.head * hd : p.part_o + at * hd;
+        T *out = (T *)p.out + row.t * p.ldo + (int64_t)row.head * hd;
+        float *po = p.part_o + at * hd;
         // rows 4 g4 + i of blocks t0 .. t0 + VD - 1: 4 VD neighbouring dimensions
 #pragma unroll
         for (int t0 = 0; t0 < C::VT; t0 += C::VD) {
@@ -882,8 +915,15 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
 #pragma unroll
                 for (int x = 0; x < C::VD; ++x) e[i * C::VD + x] = o[t0 + x][i] * inv;
 #pragma unroll
-            for (int x = 0; x < C::VD; ++x)
-                if (d + 4 * x < hd) *(vf4 *)(to + d + 4 * x) = vf4{e[4 * x], e[4 * x + 1], e[4 * x + 2], e[4 * x + 3]};
+            for (int x = 0; x < C::VD; ++x) {
+                if (d + 4 * x >= hd) continue;
+                if (whole) {
+                    T y[4] = {(T)e[4 * x], (T)e[4 * x + 1], (T)e[4 * x + 2], (T)e[4 * x + 3]};
+                    __builtin_memcpy(__builtin_assume_aligned(out + d + 4 * x, sizeof y), y, sizeof y);
+                } else {
+                    *(vf4 *)(po + d + 4 * x) = vf4{e[4 * x], e[4 * x + 1], e[4 * x + 2], e[4 * x + 3]};
+                }
+            }
         }
         if (!whole && g4 == 0) p.part_ml[at] = make_float2(m, l);
     }
@@ -893,8 +933,8 @@ __device__ __forceinline__ void attend_split(const ServeAttnParams &p, const Til
         const Row w = row_at<PREFIX>(p, q, tile * BM + wave * 16 + n, group, g);
         const Seq qs = PREFIX ? seq_at(p, (int)w.t) : q;
         float mr, lr, orow[4];
-        attend_row<float>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
-        store_row<float>(p, w.t, w.head, part, whole, true, mr, lr, orow);
+        attend_row<T>(p, qs, w.t, w.head, kb0, min(kb1, w.lim + 1), mr, lr, orow);
+        store_row<T>(p, w.t, w.head, part, whole, true, mr, lr, orow);
     }
 }
 
@@ -1219,18 +1259,18 @@ __device__ __forceinline__ void attend_few(const ServeAttnParams &p, const TileP
 }
 
 // ---- launches ----
-// A plan's rows: 16 per workgroup by the few-row form, 64 (f32) or 128 by tiles.
-enum RowForm { ROWS_FEW, ROWS_TILE };
+// A plan's rows: up to 16 per workgroup by the few-row form, tiles of 64, of 128 (16-bit types).
+enum RowForm { ROWS_FEW, ROWS_64, ROWS_128 };
 template <typename T, int HD, RowForm FORM, bool PREFIX>
 __device__ __forceinline__ void attend(const ServeAttnParams &p, const TilePlan &plan, int block, char *lds) {
     if constexpr (FORM == ROWS_FEW) attend_few<T, HD, PREFIX>(p, plan, block, lds);
-    else if constexpr (sizeof(T) == 4) attend_split<HD, PREFIX>(p, plan, block, lds);
+    else if constexpr (FORM == ROWS_64) attend_tile64<T, HD, PREFIX>(p, plan, block, lds);
     else attend_tile<T, HD, PREFIX>(p, plan, block, lds);
 }
 template <typename T, int HD, RowForm FORM>
 constexpr size_t lds_of() {
     if constexpr (FORM == ROWS_FEW) return sizeof(FewLds<HD>);
-    else if constexpr (sizeof(T) == 4) return SplitCfg<HD>::LDS;
+    else if constexpr (FORM == ROWS_64) return Tile64Cfg<T, HD>::LDS;
     else return TileCfg<T, HD>::LDS;
 }
 
@@ -1314,7 +1354,11 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     // Up to 16 rows of a sequence: the few-row form, which the tiles pass soon after (32
     // sequences of 500 to 2000 keys, 12 heads of 128: 30 rows bf16 22.4 against 20.2 us, f32
     // 38.7 against 37.3).  After a prefix it is always that: the tiles begin with key 0.
-    t.bm = avg <= 16 || key0 > 0 ? 16 : p.dtype == GAJE_DTYPE_F32 ? 64 : 128;
+    // 16-bit prompts of up to about 450 tokens have tiles of 64 rows (8 of 400, 14 heads of 64: 16.3
+    // against 20.7 us with 128; 32 of 200, 16 heads: 21.6 against 30.2; but 3 of 300 to 900, 12
+    // heads of 128: 33.7 against 28.7, one of 4000: 139 against 95).
+    const bool brief = !p.table && p.T <= 448 * seqs;
+    t.bm = avg <= 16 || key0 > 0 ? 16 : p.dtype == GAJE_DTYPE_F32 || brief ? 64 : 128;
     t.key0 = (int32_t)key0;
     // Workgroups wanted: two for each of 256 CUs; over a prefix one, where every part costs
     // partial results of all rows (64 sequences over 16000 keys: 29.1 against 38.2 us), and beside
@@ -1392,7 +1436,9 @@ template <typename T, int HD>
 int launch_head(const ServeAttnParams &p, const AttnPlan &a, hipStream_t s) {
     const int bm = a.prefix.items ? a.prefix.bm : a.keys.bm;
     if (bm == 16) return launch_form<T, HD, ROWS_FEW>(p, a, s);
-    return launch_form<T, HD, ROWS_TILE>(p, a, s);
+    if (bm == 64) return launch_form<T, HD, ROWS_64>(p, a, s);
+    if constexpr (sizeof(T) == 2) return launch_form<T, HD, ROWS_128>(p, a, s);
+    return set_error(GAJE_ERR_HIP, "attention plan of %d rows", bm);
 }
 
 template <typename T>
