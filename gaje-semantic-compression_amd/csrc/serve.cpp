@@ -31,7 +31,7 @@ int check_pages(const char *what, const gaje_hip_kv_pages *c) {
     if (c->page < 8 || c->page > 1024 || (c->page & (c->page - 1)))
         return set_error(GAJE_ERR_INVALID_ARG, "%s: page of %d positions (a power of two, 8 to 1024)", what, c->page);
     if (c->n_layer <= 0 || c->n_layer > 65535 || c->n_pages <= 0 || c->n_pages > (int64_t)1 << 26 || c->n_seq <= 0 ||
-        c->n_seq > (int64_t)1 << 20 || c->max_pages <= 0 || c->max_pages * c->page > (int64_t)1 << 24)
+        c->n_seq > 65536 || c->max_pages <= 0 || c->max_pages * c->page > (int64_t)1 << 24)
         return set_error(GAJE_ERR_INVALID_ARG, "%s: %lld layers of %lld pages, %lld sequences of up to %lld pages", what,
                          (long long)c->n_layer, (long long)c->n_pages, (long long)c->n_seq, (long long)c->max_pages);
     return GAJE_OK;
@@ -66,7 +66,7 @@ int check_rows(const char *what, const char *name, const void *p, int64_t ld, in
 }
 
 int check_count(const char *what, int64_t n_seq, int64_t T) {
-    if (n_seq < 0 || n_seq > (int64_t)1 << 20 || T < 0 || T > (int64_t)1 << 24)
+    if (n_seq < 0 || n_seq > 65536 || T < 0 || T > (int64_t)1 << 24)
         return set_error(GAJE_ERR_INVALID_ARG, "%s: %lld sequences, %lld rows", what, (long long)n_seq, (long long)T);
     return GAJE_OK;
 }

@@ -796,10 +796,11 @@ __device__ __forceinline__ void attend_tile64(const ServeAttnParams &p, const Ti
                 }
             } else {
                 qf[0][j] = a;
-                asm volatile("" : "+v"(qf[0][j]));  // (waited for here, as in the tiles of 128 rows)
             }
         }
     }
+#pragma unroll
+    for (int j = 0; j < C::STEPS; ++j) asm volatile("" : "+v"(qf[0][j]));  // (waited for here, as in the tiles of 128 rows)
     const float c = p.scale * LOG2E, slack = slack_of(c);  // (as in the tiles)
     float m = -INFINITY, l = 0.0f;
     vf4 o[C::VT];
@@ -1362,8 +1363,9 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     t.key0 = (int32_t)key0;
     // Workgroups wanted: two for each of 256 CUs; over a prefix one, where every part costs
     // partial results of all rows (64 sequences over 16000 keys: 29.1 against 38.2 us), and beside
-    // a long one half a CU's, which leaves fewer workgroups without an item.
-    t.blocks = prefix ? 8 : key0 >= 1024 ? 7 : 9;
+    // one of eight times the own keys or more half a CU's, which leaves fewer workgroups without an
+    // item.
+    t.blocks = prefix ? 8 : key0 >= 8 * most ? 7 : 9;
     // Parts of a prompt's own keys pay from 512 keys on (f32 prompts of up to 1500 tokens 67.6
     // against 75.1 us with 256, one f16 prompt of 1500 34.1 against 42.6), of a cache's from 256 (5
     // drafted tokens, f32, 37.3 against 49.4), a few rows' and a prefix's from 128.

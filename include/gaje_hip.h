@@ -297,7 +297,7 @@ typedef struct {
  * are the old ones and no page is copied.  All arrays are device memory and nothing
  * is read on the host, so that the call can be captured in a graph.
  * `workspace`: gaje_hip_kv_workspace(c) bytes, 16-byte aligned; calls that share
- * one must not overlap.  n_pages up to 2^26, n_seq up to 2^20. */
+ * one must not overlap.  n_pages up to 2^26, n_seq up to 65536. */
 int64_t gaje_hip_kv_workspace(const gaje_hip_kv_pages *c);
 int gaje_hip_kv_update(const gaje_hip_kv_pages *c, const int32_t *source, const int32_t *add, int32_t *new_table,
                        int32_t *new_len, int32_t *new_ref, int32_t *status, void *workspace,
@@ -327,11 +327,13 @@ int gaje_hip_kv_append(const gaje_hip_kv_pages *c, int64_t layer, int source_dty
  * most; ldq, ldk, ldv, ldo elements apart, so that q, k and v may be columns of
  * one fused product), row i sees rows seq_off[s]..i.  Query head h reads K/V head
  * h / (n_head / n_head_kv).  out row: softmax(scale q.k) v, written in the type.
- * seq_off: device [n_seq + 1], ascending; empty sequences are allowed, rows past
+ * seq_off: device [n_seq + 1], ascending, empty sequences allowed; rows past
  * seq_off[n_seq] of out are left as they were; out overlaps no input.  NaN and
  * infinities reach only the rows that see them (a row whose result is no number is
- * computed again key by key: correct, and slow if there are many).  head_dim a multiple of 8 up to 256, scale > 0 and at most 1e30,
- * q, k, v, out 16-byte aligned with leading dimensions that are multiples of 8, up to 2^21.
+ * computed again key by key: correct, and slow if there are many).  Up to 65536
+ * sequences, 2^24 rows, 1024 heads, 2^30 rows times heads; head_dim a multiple of 8 up
+ * to 256; scale > 0 and at most 1e30; q, k, v, out 16-byte aligned with leading
+ * dimensions that are multiples of 8, up to 2^21.
  * `workspace`: the matching _workspace() bytes, 16-byte aligned; nothing is kept
  * in it between calls, and calls that share one must not overlap. */
 int64_t gaje_hip_attention_packed_workspace(int64_t T, int64_t n_seq, int n_head, int n_head_kv, int head_dim);

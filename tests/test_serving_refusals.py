@@ -35,7 +35,7 @@ def refused(text, call, *args, **kw):
 BAD_CACHES = [(dict(page=12), "page of 12"), (dict(page=4), "page of 4"), (dict(page=2048), "page of 2048"),
               (dict(head_dim=60), "head_dim 60"), (dict(head_dim=264), "head_dim 264"), (dict(head_dim=0), "head_dim 0"),
               (dict(n_head_kv=0), "heads"), (dict(k=Mem(A + 8)), "16-byte aligned"), (dict(table=Mem(0)), "lacks an array"),
-              (dict(n_pages=(1 << 26) + 1), "pages"), (dict(n_seq=0), "sequences"), (dict(max_pages=0), "pages"),
+              (dict(n_pages=(1 << 26) + 1), "pages"), (dict(n_seq=0), "sequences"), (dict(n_seq=65537), "sequences"), (dict(max_pages=0), "pages"),
               (dict(n_layer=0), "layers"), (dict(max_pages=1 << 27), "pages")]
 
 
@@ -98,7 +98,7 @@ def packed(ops, **change):
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(scale=float("inf")), "scale"), (dict(q=Mem(A + 2)), "16-byte"), (dict(q=Mem(0)), "null q"),
     (dict(out=Mem(0)), "null out"), (dict(ldq=248), "leading"), (dict(ldk=130), "leading"), (dict(ldv=64), "leading"),
-    (dict(ldo=-256), "leading"), (dict(seq_off=Mem(0)), "null seq_off"), (dict(n_seq=-1), "sequences"),
+    (dict(ldo=-256), "leading"), (dict(seq_off=Mem(0)), "null seq_off"), (dict(n_seq=-1), "sequences"), (dict(n_seq=65537), "sequences"), (dict(T=1 << 24, n_head=128, ldq=8192, ldo=8192), "heads (2^30"),
     (dict(T=-1), "rows"), (dict(T=(1 << 24) + 1), "rows")])
 def test_packed(ops, change, text):
     refused(text, packed, ops, **change)
