@@ -1377,7 +1377,8 @@ TilePlan plan_rows(const ServeAttnParams &p, int64_t seqs, int64_t rows, int64_t
     t.splits = 1;
     while (blocks < target && t.splits < 64 && t.splits * blocks < 16 * target && t.splits * t.least < most) t.splits *= 2;
     // a sequence has at most keys / size + 1 parts per tile, and half of its keys count at least
-    t.items = tiles + (t.splits > 1 ? 2 * target / p.n_head_kv + 1 : 0);
+    // (and `splits` at most: a workgroup without an item still looks for one)
+    t.items = std::min<int64_t>(tiles * t.splits, tiles + 2 * target / p.n_head_kv + 1);
     if (t.splits == 1) t.size = INT32_MAX / 2;
     if (prefix) {
         t.size = part_size(most * blocks / PART_UNIT, (int)most, t.splits, t.least, t.blocks);
