@@ -563,29 +563,55 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
     const bool again = row.valid && row.lim >= kb0 && kb0 < kb1 && odd != 0.0f;
     uint32_t todo = (uint32_t)__ballot(again);
 
-    if (row.valid && !again) {
-        const bool seen = row.lim >= 0;
-        const int64_t at = ((int64_t)part * p.T + row.t) * p.n_head + row.head;
-        const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
-        T *out = (T *)p.out + row.t * p.ldo + (int64_t)row.head * hd;
-        float *po = p.part_o + at * hd;
+    // Registers x, x + LANE_PCS, .. hold eight neighbouring dimensions, piece p of the row.  The
+    // wave's rows go through LDS (the loop is done with it), so that its stores write whole rows:
+    // 64 prompts of 21 tokens, 48 heads of 128, 19.3 -> 12.6 us, 24 prompts of up to 2000, 12 heads,
+    // 147 -> 132, partial results over a prefix of 16000 28.2 -> 26.0.
+    constexpr int SPAN = C::NT >= 8 ? 1 : 8 / C::NT, LANE_PCS = 16 / SPAN, PER = 8 / SPAN;  // PER dimensions from each of SPAN registers
+    const float inv = !whole ? 1.0f : row.lim >= 0 ? 1.0f / l : 0.0f;
+    const int64_t at = ((int64_t)part * p.T + row.t) * p.n_head + row.head;
+    const uint64_t to = whole ? (uint64_t)(uintptr_t)((T *)p.out + row.t * p.ldo + (int64_t)row.head * hd) : (uint64_t)(uintptr_t)(p.part_o + at * hd);
+    const uint32_t fine = (uint32_t)__ballot(row.valid && !again);
+    char *const rows_lds = lds + wave * 32 * (HD == 256 ? 512 : HD * 4);
+    // WORDS: 16-byte pieces of 8 dimensions (1 of the type, 2 of f32); x0, n: the lane's pieces
+    auto put = [&](auto words, int x0, auto n_of) {
+        constexpr int WORDS = decltype(words)::value, N = decltype(n_of)::value, ROW = N * 2 * WORDS;  // 16-byte pieces of a row here
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = 8 * (i >> 2) + 4 * half + (i & 3);
-            // row r of the blocks: NT neighbouring dimensions
-            const int d = (r % C::PCS) * 8 + (r / C::PCS) * C::NT;
-            if (d >= hd) continue;
-            if (whole) {
-                T e[C::NT];
+        for (int x = 0; x < N; ++x) {
+            float e[8];
 #pragma unroll
-                for (int t = 0; t < C::NT; ++t) e[t] = (T)(o[t][i] * inv);
-                __builtin_memcpy(__builtin_assume_aligned(out + d, sizeof e), e, sizeof e);
+            for (int z = 0; z < SPAN; ++z)
+#pragma unroll
+                for (int k = 0; k < PER; ++k) e[z * PER + k] = o[k][x0 + x + z * LANE_PCS] * inv;
+            const int pc0 = 8 * (x >> 2) + 4 * half + (x & 3);
+            vu4 v[WORDS];
+            if constexpr (WORDS == 2) {
+                __builtin_memcpy(v, e, 32);
             } else {
+                T y[8];
 #pragma unroll
-                for (int t = 0; t < C::NT; ++t) po[d + t] = o[t][i];
+                for (int k = 0; k < 8; ++k) y[k] = (T)e[k];
+                __builtin_memcpy(v, y, 16);
             }
+#pragma unroll
+            for (int h = 0; h < WORDS; ++h) *(vu4 *)(rows_lds + (l32 * ROW + ((pc0 * WORDS + h) ^ (l32 & (ROW - 1) & 15))) * 16) = v[h];
         }
-        if (!whole && half == 0) p.part_ml[at] = make_float2(m, l);
+#pragma unroll
+        for (int x = 0; x < ROW / 2; ++x) {  // 64 / ROW rows of a store
+            const int r = x * (64 / ROW) + lane / ROW, w = lane % ROW, d = (x0 * 2 + w / WORDS) * 8;
+            const uint32_t lo = __shfl((uint32_t)to, r, WAVE), hi = __shfl((uint32_t)(to >> 32), r, WAVE);
+            const vu4 v = *(const vu4 *)(rows_lds + (r * ROW + (w ^ (r & (ROW - 1) & 15))) * 16);
+            if ((fine >> r & 1) && d < hd) *(vu4 *)((char *)(uintptr_t)((uint64_t)hi << 32 | lo) + x0 * 2 * WORDS * 16 + w * 16) = v;
+        }
+    };
+    using std::integral_constant;
+    if (whole) {
+        put(integral_constant<int, 1>{}, 0, integral_constant<int, LANE_PCS>{});
+    } else {
+        constexpr int N = HD == 256 ? LANE_PCS / 2 : LANE_PCS;
+#pragma unroll
+        for (int x0 = 0; x0 < LANE_PCS; x0 += N) put(integral_constant<int, 2>{}, x0, integral_constant<int, N>{});
+        if (row.valid && !again && half == 0) p.part_ml[at] = make_float2(m, l);
     }
     while (todo) {
         const int n = __builtin_ctz(todo);
