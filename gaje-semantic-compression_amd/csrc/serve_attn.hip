@@ -560,7 +560,13 @@ __device__ __forceinline__ void attend_tile(const ServeAttnParams &p, const Tile
 #pragma unroll
         for (int i = 0; i < 16; ++i) odd = fmaf(o[t][i], 0.0f, odd);
     odd += __shfl_xor(odd, 32, WAVE);
-    const bool again = row.valid && row.lim >= kb0 && kb0 < kb1 && odd != 0.0f;
+    const bool again = row.valid && row.lim >= kb0 && odd != 0.0f;
+    if (odd != 0.0f && !again) {  // (the row sees none of these keys)
+#pragma unroll
+        for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    }
     uint32_t todo = (uint32_t)__ballot(again);
 
     // Registers x, x + LANE_PCS, .. hold eight neighbouring dimensions, piece p of the row.  The
@@ -924,7 +930,13 @@ __device__ __forceinline__ void attend_tile64(const ServeAttnParams &p, const Ti
         for (int i = 0; i < 4; ++i) odd = fmaf(o[t][i], 0.0f, odd);
     odd += __shfl_xor(odd, 16, WAVE);
     odd += __shfl_xor(odd, 32, WAVE);
-    const bool again = row.valid && row.lim >= kb0 && kb0 < kb1 && odd != 0.0f;
+    const bool again = row.valid && row.lim >= kb0 && odd != 0.0f;
+    if (odd != 0.0f && !again) {
+#pragma unroll
+        for (int t = 0; t < C::VT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
+    }
     uint32_t todo = (uint32_t)__ballot(again) & 0xffffu;
     if (row.valid && !again) {
         const bool seen = row.lim >= 0;
@@ -1226,7 +1238,7 @@ __device__ __forceinline__ void attend_few(const ServeAttnParams &p, const TileP
 #pragma unroll
         for (int t = 0; t < C::VW; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) joined[wave][l16][(4 * g4 + i) * C::VW + t] = m == -INFINITY ? 0.0f : o[t][i] * shrink;
+            for (int i = 0; i < 4; ++i) joined[wave][l16][(4 * g4 + i) * C::VW + t] = o[t][i] * shrink;
     }
     __syncthreads();
     // 256 / BM threads per row
@@ -1255,7 +1267,11 @@ __device__ __forceinline__ void attend_few(const ServeAttnParams &p, const TileP
         bad = fmaf(v[x].x, 0.0f, bad), bad = fmaf(v[x].y, 0.0f, bad), bad = fmaf(v[x].z, 0.0f, bad), bad = fmaf(v[x].w, 0.0f, bad);
     }
     // (as in the tiles: a row whose result is no number is computed again, key by key)
-    if (bad != 0.0f && row.valid && row.lim >= kb0 && kb0 < kb1) odd[r] = 1;
+    if (bad != 0.0f) {
+        if (row.valid && row.lim >= kb0) odd[r] = 1;
+        else
+            for (auto &x : v) x = make_float4(0, 0, 0, 0);
+    }
     __syncthreads();
     if (row.valid && !odd[r]) {
         const bool seen = row.lim >= 0;
@@ -1345,7 +1361,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ServeAttnParams p, TileP
     for (int i = lane / LPP; i < parts; i += SIDE) {
         const float2 ml = p.part_ml[place(i)];
         const vf4 po = *(const vf4 *)(p.part_o + place(i) * hd + min(d, hd - 4));
-        // (a part without a key that the row sees: -inf, 0)
+        // (a part without a key that the row sees: -inf, and zeros; one whose scores are -inf or no
+        // numbers: -inf, and sums whose NaN the weight 0 lets through)
         const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(ml.x, c, -base));
         l = fmaf(w, ml.y, l);
 #pragma unroll

@@ -672,3 +672,119 @@ def test_scores_of_minus_infinity(ops, dtype):
     q, k, v = (x[:, a * hd:b * hd].reshape(n, b - a, hd) for a, b in ((0, H), (H, H + G), (H + G, H + 2 * G)))
     ref, mass, top = R.attend(q[40:], k[40:], v[40:], 0, 0.1)
     close(out[40:], ref, R.bound(dtype, ref, mass, top, hd, n))
+
+
+def all_or_none(out, want):
+    """Rows of which a True in want says that they are no numbers throughout, and the others' rows."""
+    nan = torch.isnan(out.float().cpu()).reshape(out.shape[0], -1, want.shape[-1])
+    assert bool((nan.all(2) == want.all(2)).all()) and bool((nan.any(2) == want.any(2)).all()), (nan.sum(2), want.sum(2))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("form", ["packed", "tokens", "prefix-few", "prefix-tiles"])
+def test_keys_without_a_number_fill_a_part(ops, dtype, form):
+    """Keys cut into parts, of which one holds no score that is a number: rows that see it are NaN."""
+    H, G, hd, n = 6, 2, 64, 1100
+    for first in (512, 1024):
+        if form == "packed":
+            x = normal((n, (H + 2 * G) * hd), dtype, seed=n)
+            x[first:, H * hd:(H + 1) * hd] = math.nan
+            out = run_packed(ops, x.cuda(), [n], H, G, hd, 0.1)
+            want = torch.zeros(n, H, hd, dtype=torch.bool)
+            want[first:, :3] = True
+            all_or_none(out, want)
+            continue
+        seqs = 24 if form == "prefix-tiles" else 3
+        lengths = [n + 20 - 9 * s for s in range(seqs - 1)] + [first]
+        c = R.Cache(lengths, 16, G, hd, dtype, seed=2)
+        for s, m in enumerate(lengths):
+            for pool in (c.k, c.v):
+                x = c.rows(pool, 0, s, m).clone()
+                shared = min(m, n)
+                x[:shared] = c.rows(pool, 0, 0, shared)
+                if pool is c.k:
+                    x[first:n, 0] = math.nan
+                c.write(pool, 0, s, x)
+        _, h = device_cache(ops, c)
+        q = normal((seqs, H * hd), dtype, seed=3).cuda()
+        prefix = n if form.startswith("prefix") else 0
+        out = run_prefix(ops, h, q, prefix, H, 0.12, c.table[0].clone().cuda()) if prefix else run_paged(ops, h, q, [1] * seqs, H, 0.12)
+        want = torch.zeros(seqs, H, hd, dtype=torch.bool)
+        want[[s for s, m in enumerate(lengths) if m > first], :3] = True
+        all_or_none(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("form", ["packed", "rows", "drafts", "prefix-few", "prefix-tiles"])
+def test_parts_a_row_does_not_see(ops, dtype, form):
+    """Values that are no numbers in a part of the keys of which a row sees none."""
+    H, G, hd, n = 6, 2, 64, 1100
+    for first in (512, 1024):
+        if form == "packed":
+            x = normal((n, (H + 2 * G) * hd), dtype, seed=n)
+            x[first:, (H + G) * hd:(H + G + 1) * hd] = math.nan
+            out = run_packed(ops, x.cuda(), [n], H, G, hd, 0.1)
+            want = torch.zeros(n, H, hd, dtype=torch.bool)
+            want[first:, :3] = True
+            all_or_none(out, want)
+            continue
+        seqs = 24 if form == "prefix-tiles" else 3
+        rows = {"rows": [60] * seqs, "drafts": [5] * seqs}.get(form, [1] * seqs)
+        lengths = [n - 9 * s for s in range(seqs - 1)] + [first] if form.startswith("prefix") else [first + 4, first + 1, first + 30]
+        c = R.Cache(lengths, 16, G, hd, dtype, seed=2)
+        for s, m in enumerate(lengths):
+            for pool in (c.k, c.v):
+                x = c.rows(pool, 0, s, m).clone()
+                if form.startswith("prefix"):
+                    x[:] = c.rows(pool, 0, 0, m)
+                if pool is c.v:
+                    x[first:, 0] = math.nan
+                c.write(pool, 0, s, x)
+        _, h = device_cache(ops, c)
+        q = normal((sum(rows), H * hd), dtype, seed=3).cuda()
+        out = run_prefix(ops, h, q, n, H, 0.12, c.table[0].clone().cuda()) if form.startswith("prefix") else run_paged(ops, h, q, rows, H, 0.12)
+        want = torch.zeros(sum(rows), H, hd, dtype=torch.bool)
+        at = 0
+        for s, r in enumerate(rows):
+            for i in range(r):
+                want[at + i, :3] = lengths[s] - r + i >= first
+            at += r
+        all_or_none(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [4, 9, 80])
+def test_rows_without_a_position(ops, dtype, rows):
+    """Rows in front of a sequence's first position are zeros, whatever its keys and values hold."""
+    H, G, hd, length = 6, 2, 64, rows - 2
+    c = R.Cache([length], 16, G, hd, dtype, seed=6)
+    for pool in (c.k, c.v):
+        x = c.rows(pool, 0, 0, length).clone()
+        x[1, 0] = math.nan
+        c.write(pool, 0, 0, x)
+    _, h = device_cache(ops, c)
+    q = normal((rows, H * hd), dtype, seed=3).cuda()
+    out = run_paged(ops, h, q, [rows], H, 0.12).cpu().reshape(rows, H, hd)
+    assert bool((out[:2] == 0).all())
+    want = torch.zeros(rows, H, hd, dtype=torch.bool)
+    want[3:, :3] = True
+    all_or_none(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 30])
+def test_values_without_a_number_at_weight_zero(ops, dtype, rows):
+    """Keys whose score is -inf have weight 0, and 0 times a NaN value is NaN in its dimension."""
+    H, G, hd, n = 6, 2, 64, 1100
+    c = R.Cache([n], 16, G, hd, dtype, seed=6)
+    k, v = c.rows(c.k, 0, 0, n).abs(), c.rows(c.v, 0, 0, n).clone()
+    k[:700] = -math.inf
+    v[40, 0, 9] = v[600, 1, 11] = math.nan
+    c.write(c.k, 0, 0, k)
+    c.write(c.v, 0, 0, v)
+    _, h = device_cache(ops, c)
+    q = (normal((rows, H * hd), dtype, seed=3).abs() + 0.5).cuda()  # positive queries
+    out = run_paged(ops, h, q, [rows], H, 0.12)
+    nan = torch.zeros(rows, H, hd, dtype=torch.bool)
+    nan[:, :3, 9] = nan[:, 3:, 11] = True
+    assert torch.equal(torch.isnan(out.cpu().float()).reshape(rows, H, hd), nan)
