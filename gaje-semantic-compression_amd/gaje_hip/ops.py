@@ -265,6 +265,10 @@ def kv_pages(k, v, table, length, ref, *, n_layer: int, n_pages: int, page: int,
     return c
 
 
+def _space(workspace):
+    return (None, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+
+
 def kv_workspace(cache: KvPages) -> int:
     return int(lib().gaje_hip_kv_workspace(cache))
 
@@ -274,13 +278,12 @@ def kv_update(cache: KvPages, new_table, new_length, new_ref, status, workspace,
     """Slots forked, freed, cut and grown: slot d becomes old slot source[d] (-1: empty), its
     length changed by add[d]; the new arrays receive the result (gaje_hip_kv_update)."""
     check(lib().gaje_hip_kv_update(cache, _p(source), _p(add), new_table.ptr, new_length.ptr, new_ref.ptr, status.ptr,
-                                   workspace.ptr, workspace.nbytes, stream))
+                                   *_space(workspace), stream))
 
 
 def kv_compact(cache: KvPages, new_table, new_ref, n_live, workspace, stream=None) -> None:
     """The pages in use moved to the front of the pool (gaje_hip_kv_compact)."""
-    check(lib().gaje_hip_kv_compact(cache, new_table.ptr, new_ref.ptr, n_live.ptr, workspace.ptr, workspace.nbytes,
-                                    stream))
+    check(lib().gaje_hip_kv_compact(cache, new_table.ptr, new_ref.ptr, n_live.ptr, *_space(workspace), stream))
 
 
 def kv_append(cache: KvPages, layer: int, k, ldk: int, v, ldv: int, seq_off, T: int, source: str = "f32",
@@ -297,8 +300,7 @@ def attention_packed(q, ldq: int, k, ldk: int, v, ldv: int, seq_off, n_seq: int,
                      head_dim: int, scale: float, out, ldo: int, workspace, dtype: str = "f32", stream=None) -> None:
     """Causal GQA attention of n_seq prompts packed row after row (gaje_hip_attention_packed)."""
     check(lib().gaje_hip_attention_packed(DTYPES[dtype], q.ptr, ldq, k.ptr, ldk, v.ptr, ldv, seq_off.ptr, n_seq, T,
-                                          n_head, n_head_kv, head_dim, scale, out.ptr, ldo, workspace.ptr,
-                                          workspace.nbytes, stream))
+                                          n_head, n_head_kv, head_dim, scale, out.ptr, ldo, *_space(workspace), stream))
 
 
 def attention_paged_workspace(cache: KvPages, T: int, n_head: int) -> int:
@@ -310,7 +312,7 @@ def attention_paged(q, ldq: int, cache: KvPages, layer: int, seq_off, T: int, n_
     """Causal GQA attention of each sequence's last rows over its cached pages
     (gaje_hip_attention_paged): single tokens, drafted tokens, a prompt's next chunk."""
     check(lib().gaje_hip_attention_paged(q.ptr, ldq, cache, layer, seq_off.ptr, T, n_head, scale, out.ptr, ldo,
-                                         workspace.ptr, workspace.nbytes, stream))
+                                         *_space(workspace), stream))
 
 
 def attention_prefix_workspace(cache: KvPages, prefix_len: int, n_head: int) -> int:
@@ -321,8 +323,8 @@ def attention_prefix(q, ldq: int, cache: KvPages, layer: int, prefix_table, pref
                      out, ldo: int, workspace, stream=None) -> None:
     """One token of every sequence over a prefix they all share, read once for all, and
     each sequence's own positions after it (gaje_hip_attention_prefix)."""
-    check(lib().gaje_hip_attention_prefix(q.ptr, ldq, cache, layer, prefix_table.ptr, prefix_len, n_head, scale,
-                                          out.ptr, ldo, workspace.ptr, workspace.nbytes, stream))
+    check(lib().gaje_hip_attention_prefix(q.ptr, ldq, cache, layer, _p(prefix_table), prefix_len, n_head, scale,
+                                          out.ptr, ldo, *_space(workspace), stream))
 
 
 def kwta(scores: DeviceBuffer, n: int, k: int, stream=None):

@@ -156,3 +156,18 @@ def test_struct_layout(tmp_path):
     subprocess.run(["gcc", "-std=c11", "-I", os.path.join(REPO, "include"), str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
     got = [int(x) for x in subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [ctypes.sizeof(_lib.KvPages)] + [getattr(_lib.KvPages, f).offset for f in names]
+
+
+def test_arguments_that_may_be_missing(ops):
+    """No workspace where none is needed, no prefix table without a prefix; refused where they are."""
+    from gaje_hip import GajeError
+    c, m = cache(ops), Mem()
+    packed(ops, T=0, workspace=None)
+    ops.attention_paged(m, 256, c, 0, m, 0, 4, 0.1, m, 256, None)
+    assert ops.attention_packed_workspace(8190, 1, 4, 2, 64) > 0
+    refused("workspace", packed, ops, T=8190, n_seq=1, workspace=None)
+    refused("workspace", ops.kv_update, c, Mem(64 * A), Mem(65 * A), Mem(66 * A), m, None)
+    refused("workspace", ops.kv_compact, c, Mem(64 * A), Mem(66 * A), m, None)
+    refused("prefix of", ops.attention_prefix, m, 256, c, 0, None, 16, 4, 0.1, m, 256, m)
+    with pytest.raises(GajeError, match="null q"):
+        ops.attention_prefix(Mem(0), 256, c, 0, None, 0, 4, 0.1, m, 256, m)
