@@ -165,7 +165,7 @@ def test_arguments_that_may_be_missing(ops):
     packed(ops, T=0, workspace=None)
     ops.attention_paged(m, 256, c, 0, m, 0, 4, 0.1, m, 256, None)
     assert ops.attention_packed_workspace(8190, 1, 4, 2, 64) > 0
-    refused("workspace", packed, ops, T=8190, n_seq=1, workspace=None)
+    refused("workspace", packed, ops, T=8190, n_seq=1, workspace=None, dtype="f16")
     refused("workspace", ops.kv_update, c, Mem(64 * A), Mem(65 * A), Mem(66 * A), m, None)
     refused("workspace", ops.kv_compact, c, Mem(64 * A), Mem(66 * A), m, None)
     refused("prefix of", ops.attention_prefix, m, 256, c, 0, None, 16, 4, 0.1, m, 256, m)
