@@ -12,7 +12,7 @@
 // instructions) and attend_few (up to 16 rows, the keys split over the waves).  The keys of a
 // tile are cut into parts where there are few tiles; attn_join_kernel joins what they leave.
 // Measured, as launched in a graph:
-//   attend_tile    one prompt of 8190, 32/8 heads of 128, f16: 610 us, 900 TFLOP/s
+//   attend_tile    one prompt of 8190, 32/8 heads of 128, f16: 620 us, 890 TFLOP/s
 //   attend_tile64  4 f32 prompts of 970 to 1930, 12/2 heads of 128: 258 us, 143 TFLOP/s (f32
 //                  products of a library: 154)
 //   attend_few     512 sequences of 1000 keys, 12/2 heads of 128, bf16: 97 us, 5.4 TB/s
