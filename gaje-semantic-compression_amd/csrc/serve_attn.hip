@@ -266,8 +266,33 @@ __device__ __forceinline__ bool find_item(const ServeAttnParams &p, const TilePl
         }
         size = part_size(total * p.n_head_kv, longest, plan.splits, plan.least, plan.blocks);
     }
-    int base = 0;
-    for (int s0 = 0; s0 < n_seq; s0 += WAVE) {
+    int base = 0, begin = 0;
+    if (plan.splits == 1 && n_seq > 4 * WAVE) {
+        // Of many sequences the eight that hold the item are found first, eight per lane (4096 of 200
+        // cached keys, one token each, 12/2 heads of 128, bf16: 561 -> 400 us).
+        constexpr int RUN = 8;
+        for (; begin < n_seq; begin += WAVE * RUN) {
+            const int left = n_seq - begin, first = min(lane * RUN, left);
+            int at[RUN + 1], sum = 0;
+#pragma unroll
+            for (int i = 0; i <= RUN; ++i) {
+                const int s = min(first + i, left);
+                at[i] = p.seq_off ? min(max(p.seq_off[begin + s], 0), (int)p.T) : s;
+            }
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) sum += (int)(((int64_t)max(at[i + 1] - at[i], 0) * group + plan.bm - 1) >> shift);
+            const int incl = wave_scan(sum);
+            const uint64_t past = __ballot(base + incl > b);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                base += __builtin_amdgcn_readlane(incl - sum, l);
+                begin += l * RUN;
+                break;
+            }
+            base += __builtin_amdgcn_readlane(incl, WAVE - 1);
+        }
+    }
+    for (int s0 = begin; s0 < n_seq; s0 += WAVE) {
         if (plan.size || n_seq > WAVE) look(s0);
         const int parts = plan.splits == 1 ? 1 : (int)((uint32_t)max(cut - 1, 0) / (uint32_t)size) + 1;
         const int cnt = tiles * parts, incl = wave_scan(cnt), total = __builtin_amdgcn_readlane(incl, WAVE - 1);

@@ -788,3 +788,21 @@ def test_values_without_a_number_at_weight_zero(ops, dtype, rows):
     nan = torch.zeros(rows, H, hd, dtype=torch.bool)
     nan[:, :3, 9] = nan[:, 3:, 11] = True
     assert torch.equal(torch.isnan(out.cpu().float()).reshape(rows, H, hd), nan)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seqs", [257, 600, 1100])
+def test_tokens_of_many_sequences(ops, dtype, seqs):
+    """One token each of some hundred sequences: over their own pages, some idle, and after a prefix."""
+    H, G, hd, prefix = 6, 2, 32, 20
+    lengths = [prefix + (s * 13) % 50 for s in range(seqs)]
+    c = R.Cache(lengths, 16, G, hd, dtype, seed=seqs)
+    for s in range(1, seqs):
+        for pool in (c.k, c.v):
+            c.write(pool, 0, s, c.rows(pool, 0, 0, prefix).clone())
+    _, h = device_cache(ops, c)
+    q = normal((seqs, H * hd), dtype, seed=3).cuda()
+    out = run_prefix(ops, h, q, prefix, H, 0.2, c.table[0].clone().cuda())
+    check_paged(c, q, out, [1] * seqs, H, 0.2)
+    rows = [int(s % 3 != 0) for s in range(seqs)]
+    check_paged(c, q[:sum(rows)], run_paged(ops, h, q[:sum(rows)], rows, H, 0.2), rows, H, 0.2)
